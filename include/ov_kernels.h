@@ -206,6 +206,106 @@ int ov_attention_varlen_items(const uint16_t* qkv, size_t ld_qkv, size_t rows,
                               size_t heads, size_t kv_heads, size_t head_dim, float scale,
                               uint16_t* out, size_t ld_out, ov_stream_t stream);
 
+/* ------------------------------------------------- 8-bit key/value cache */
+
+/* A paged cache of keys and values in 8 bits.  No counterpart in the
+ * reference, which recomputes every key and value in every step: it is an
+ * addition of this library for callers that keep a prompt's keys and values,
+ * or decode token by token.
+ *
+ * A page holds `page_tokens` consecutive tokens of one sequence; per page and
+ * kv head it has int8 codes [page_tokens][head_dim] and one float32 scale,
+ * for keys and for values apart.  A code c stands for c * scale.  Token t of
+ * sequence s lies in page page_table[s * max_pages + t / page_tokens], slot
+ * t % page_tokens.  Sequences may share pages that they only read.
+ * All arrays are DEVICE memory; the struct itself is read during the call.
+ *   keys, values   int8 [pages][kv_heads][page_tokens][head_dim], 16-byte aligned
+ *   *_scales       float [pages][kv_heads]
+ *   page_table     int32 [num_seqs][max_pages]
+ * page_tokens is 16, 32, 64 or 128; head_dim must be 128;
+ * pages * kv_heads * page_tokens stays below 2^31 (256 GB of keys).
+ *
+ * Checks: sizes, alignment and that a call's tensors lie on the current
+ * device are checked on the host (OV_ERR_INVALID).  What only the device sees
+ * is skipped and reported as OV_DEVICE_BAD_ARGUMENT by ov_take_device_errors:
+ * a page outside [0, pages), a token past max_pages * page_tokens, a negative
+ * start or length, row bounds that decrease, leave [0, rows] or name more
+ * than max_rows rows.  The entry points allocate nothing and may be captured
+ * into a graph after a first call on the device. */
+typedef struct {
+  int8_t* keys;
+  int8_t* values;
+  float* key_scales;
+  float* value_scales;
+  const int32_t* page_table;
+  size_t pages;
+  size_t page_tokens;
+  size_t kv_heads;
+  size_t head_dim;
+  size_t num_seqs;
+  size_t max_pages;
+} ov_kv_cache;
+
+/* Quantises packed rows into the cache.  Sequence s takes the rows
+ * [cu_rows[s], cu_rows[s + 1]) of k and v (half, kv head h in columns
+ * [h * head_dim, (h + 1) * head_dim), row strides ld_k / ld_v in elements,
+ * multiples of 8; pointers 16-byte aligned) as its tokens starts[s],
+ * starts[s] + 1, ...  cu_rows (num_seqs + 1 entries) and starts (num_seqs)
+ * are device int32; max_rows bounds the rows of one sequence.
+ *
+ * A page's scale is the largest |x| written / 127, and at least its old
+ * scale when the page keeps tokens before starts[s]; if it grows, the kept
+ * codes are rounded onto the new grid.  So a value is off by half a scale,
+ * and by half a scale more each time its page's scale grew after it was
+ * written.  What a page held from starts[s] on counts as gone: a sequence
+ * ends with its last written token, and rewriting a tail (starts below the
+ * current end) is allowed.  Slots behind the last written token keep their
+ * codes.  A page with a NaN or an infinity among its rows gets a NaN scale,
+ * hence reads back as NaN, until it is rewritten from its first slot.
+ * A page may be written by one sequence of a call only. */
+int ov_kv_cache_write(const ov_kv_cache* cache, const uint16_t* k, size_t ld_k, const uint16_t* v,
+                      size_t ld_v, size_t rows, const int32_t* cu_rows, const int32_t* starts,
+                      size_t max_rows, ov_stream_t stream);
+
+/* The inverse gather: row cu_rows[s] + i of k and v becomes half(code * scale)
+ * of token starts[s] + i of sequence s.  Rows outside every sequence, and
+ * rows of tokens that the page table does not cover, are left as they are. */
+int ov_kv_cache_read(const ov_kv_cache* cache, const int32_t* cu_rows, const int32_t* starts,
+                     size_t rows, size_t max_rows, uint16_t* k, size_t ld_k, uint16_t* v,
+                     size_t ld_v, ov_stream_t stream);
+
+/* Grouped-query attention of each sequence's rows over its cache, the
+ * cached form of ov_attention_varlen: for row i of the n rows of sequence s,
+ * head h and kv head h / (heads / kv_heads),
+ *   out = softmax(scale * q . K^T) V
+ * over the sequence's first lengths[s] tokens, or with `causal` over tokens
+ * [0, lengths[s] - n + i]: the rows are the sequence's last n tokens, already
+ * in the cache.  A row that sees no token gives zeros.  Rows outside every
+ * sequence are left as they are.
+ * q is half [rows][ld_q], head h in columns [h * head_dim, ...), out likewise
+ * with ld_out (strides multiples of 8, pointers 16-byte aligned); cu_rows,
+ * lengths device int32; max_rows and max_length bound rows and lengths of
+ * one sequence (a longer length is cut there and reported); scale > 0.
+ *
+ * K and V enter the products as their codes, exact in half; the scales are
+ * applied to the float32 scores and, as log2(value scale), inside the
+ * exponent, so a probability is rounded to half once, relative to the row's
+ * largest (probability x value scale).  Softmax statistics are float32.
+ *
+ * With few rows a sequence's tokens are split over several CTAs whose parts
+ * are joined in a fixed order: results do not depend on timing.  That needs
+ * `workspace` (16-byte aligned) of ov_attention_kv_cache_workspace_bytes;
+ * with a smaller one or NULL each row runs on one CTA.  Zero it once before
+ * its first use (every call leaves its counters zero); calls sharing a
+ * workspace must not overlap, captured ones included. */
+int ov_attention_kv_cache(const ov_kv_cache* cache, const uint16_t* q, size_t ld_q, size_t rows,
+                          const int32_t* cu_rows, size_t max_rows, const int32_t* lengths,
+                          size_t max_length, size_t heads, int causal, float scale, uint16_t* out,
+                          size_t ld_out, void* workspace, size_t workspace_bytes,
+                          ov_stream_t stream);
+size_t ov_attention_kv_cache_workspace_bytes(const ov_kv_cache* cache, size_t rows,
+                                             size_t max_rows, size_t max_length, size_t heads);
+
 /* ------------------------------------------------------ decoding tail */
 
 /* generator_kernels.hpp:58-66 (Score).  logits rows [0, frames) are
@@ -216,6 +316,30 @@ int ov_attention_varlen_items(const uint16_t* qkv, size_t ld_qkv, size_t rows,
 int ov_score(const float* logits, size_t ld, size_t frames, size_t codebooks, size_t vocab,
              uint32_t mask_id, float guidance, int32_t* prediction, float* confidence,
              ov_stream_t stream);
+
+/* Log probabilities of given tokens under logits, beside ov_score (which
+ * picks tokens).  No counterpart in the reference.  Row r of `logits` (type
+ * OV_LOGITS_*, row stride ld in elements) holds `codebooks` groups of `vocab`
+ * values; for each item [codebook][row], with p = softmax of its group:
+ *   logprob       log p[target]
+ *   rank          tokens ahead of the target (greater logit, or an equal one
+ *                 with a lower index); 0 for the most likely
+ *   entropy       -sum p log p, in nats
+ *   top_ids, top_logprobs  [codebook][row][top_k]: the top_k most likely,
+ *                 equal ones by lower index
+ * targets is int32 [codebook][row]; a negative target asks for nothing:
+ * logprob 0, rank -1; one >= vocab the same, reported as
+ * OV_DEVICE_BAD_ARGUMENT.  entropy and rank may be NULL, the top_* too when
+ * top_k is 0.  A closed token has logit -inf: probability 0, and it is an
+ * alternative only when fewer than top_k are open.  A group with a NaN or
+ * +inf, or with nothing above -inf, has no distribution: NaN, rank and ids -1.
+ * top_k is at most 32 and at most vocab, vocab at most 2^20.  Sums are
+ * float32, whatever the logits' type. */
+enum { OV_LOGITS_F32 = 0, OV_LOGITS_F16 = 1 };
+int ov_token_logprobs(const void* logits, int logits_type, size_t ld, size_t rows,
+                      size_t codebooks, size_t vocab, const int32_t* targets, size_t top_k,
+                      float* logprob, float* entropy, int32_t* rank, int32_t* top_ids,
+                      float* top_logprobs, ov_stream_t stream);
 
 /* Noise sources of the position choice (decoding.cpp:82-87). */
 enum {

@@ -30,6 +30,9 @@ OV_EPI_SWIGLU_F16 = 2
 OV_EPI_QKNORM_ROPE_F16 = 3
 OV_SWIGLU_GROUP = 64
 
+OV_LOGITS_F32 = 0
+OV_LOGITS_F16 = 1
+
 OV_NOISE_NONE = 0
 OV_NOISE_DEVICE = 1
 OV_NOISE_BUFFER = 2
@@ -80,6 +83,14 @@ class EpilogueArgs(Structure):
                 ("rope_cos", c_void_p), ("rope_sin", c_void_p), ("max_positions", c_int32),
                 ("heads", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32),
                 ("epsilon", c_float)]
+
+
+class KvCache(Structure):
+    """ov_kv_cache (include/ov_kernels.h); the pointers are device addresses."""
+    _fields_ = [("keys", c_void_p), ("values", c_void_p), ("key_scales", c_void_p),
+                ("value_scales", c_void_p), ("page_table", c_void_p), ("pages", c_size_t),
+                ("page_tokens", c_size_t), ("kv_heads", c_size_t), ("head_dim", c_size_t),
+                ("num_seqs", c_size_t), ("max_pages", c_size_t)]
 
 
 class CodecConfigC(Structure):
@@ -154,6 +165,12 @@ SIGNATURES: dict[str, tuple] = {
     "ov_attention_varlen": (c_int, [_P, _S, _S, _P, _S, _S, _S, _S, _S, c_float, _P, _S, _P]),
     "ov_attention_varlen_items": (c_int, [_P, _S, _S, _P, _S, _S, _P, _S, c_int, _S, _S, _S,
                                           c_float, _P, _S, _P]),
+    "ov_kv_cache_write": (c_int, [POINTER(KvCache), _P, _S, _P, _S, _S, _P, _P, _S, _P]),
+    "ov_kv_cache_read": (c_int, [POINTER(KvCache), _P, _P, _S, _S, _P, _S, _P, _S, _P]),
+    "ov_attention_kv_cache": (c_int, [POINTER(KvCache), _P, _S, _S, _P, _S, _P, _S, _S, c_int,
+                                      c_float, _P, _S, _P, _S, _P]),
+    "ov_attention_kv_cache_workspace_bytes": (c_size_t, [POINTER(KvCache), _S, _S, _S, _S]),
+    "ov_token_logprobs": (c_int, [_P, c_int, _S, _S, _S, _S, _P, _S, _P, _P, _P, _P, _P, _P]),
     "ov_score": (c_int, [_P, _S, _S, _S, _S, c_uint32, c_float, _P, _P, _P]),
     "ov_select_positions": (c_int, [_P, _P, _S, _S, _S, c_float, c_float, c_int, _P, c_uint64,
                                     c_int32, c_uint32, _P, _P, _P, _S, _S, _S, _P]),
