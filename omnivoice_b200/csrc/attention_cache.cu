@@ -8,6 +8,7 @@
 // is p_j b_j relative to the row's largest, so out = (sum P_j V'_j) /
 // (sum P_j / b_j), and both products take the codes themselves, which are
 // exact in half.
+#include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -42,9 +43,25 @@ struct CacheAttnArgs {
   uint32_t* err;
 };
 
-// Stands for a value scale of 0: its codes add nothing, its tokens still
+// Stands for a value scale below it, 0 above all: such codes add nothing
+// that a half could hold (127 * 2^-31 is its least value), but their tokens
 // count in the denominator.  Below the least scale of a nonzero half page.
-constexpr float kZeroScale = 0x1.0p-31f;
+constexpr float kLeastScale = 0x1.0p-31f;
+
+// log2 and inverse of a value scale.  A NaN one (or a negative one, which
+// none is) makes the exponent NaN where it is seen, and must not reach a sum
+// where it is not.
+__device__ __forceinline__ void ValueScale(float scale, float* shift, float* inverse) {
+  const float b = scale >= 0.0f && scale < kLeastScale ? kLeastScale : scale;
+  *shift = __log2f(b);
+  *inverse = b == b ? __fdividef(1.0f, b) : 0.0f;
+}
+
+__device__ __forceinline__ float Exp2Approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 // Tokens of a sequence, bounded by what the call announced.
 __device__ __forceinline__ int SequenceLength(const CacheAttnArgs& a, int seq) {
@@ -81,9 +98,8 @@ __global__ void __launch_bounds__(128) cache_attention_row_kernel(const CacheAtt
     if (page < 0) continue;
     const int64_t at = static_cast<int64_t>(page) * a.cache.kv_heads + kv_head;
     const float c = a.scale_log2 * a.cache.key_scales[at];
-    float b = a.cache.value_scales[at];
-    b = b == 0.0f ? kZeroScale : b;
-    const float shift = log2f(b), inverse = 1.0f / b;
+    float shift, inverse;
+    ValueScale(a.cache.value_scales[at], &shift, &inverse);
     const int64_t tile = CacheTile(a.cache, page, kv_head) + lane * 4;
     const int n = min(page_tokens, seen - first);
     for (int j = 0; j < n; ++j) {
@@ -105,6 +121,603 @@ __global__ void __launch_bounds__(128) cache_attention_row_kernel(const CacheAtt
       make_uint2(pack_half2(o[0] * inv, o[1] * inv), pack_half2(o[2] * inv, o[3] * inv));
 }
 
+// ------------------------------------------- few rows: keys streamed by warps
+//
+// Up to 16 query rows share a kv head (tokens x heads of the group), so the
+// products have M or N of 8 to 16 and the time is that of reading the codes.
+// Tensor memory and its 128-row tiles would be mostly padding; here the keys
+// take the 16-row side of mma.sync instead, S^T = K Q^T and O^T = V^T P^T,
+// and the rows its 8-column side.
+//
+// Work is cut into units of 32 keys of one (sequence, kv head), numbered
+// along sequences and heads, and every CTA takes the same count of
+// consecutive units, whatever the lengths.  Each of its 8 warps streams every
+// eighth unit through a ring of its own (TMA, 128B swizzle), with its own
+// running maximum, sums and O; they join in shared memory where the CTA's
+// range leaves a (sequence, head).  One that spans several CTAs is joined by
+// the last of them to arrive, over the parts in CTA order.
+//
+// Fragments straight from the swizzled tiles: lane 4g + c, MMA row g is key
+// kappa(g) of a slab of 16 (and 8 + kappa(g)).  kappa puts neighbouring g
+// into different halves of a 128-byte line, so that K reads (16 bytes of key
+// g, dims 64 j + 16 c) and V reads (16 bytes of key kappa(2c), dims 16 g) are
+// both free of bank conflicts.  The order of dims in the first product, and
+// of keys in the second, is the same for both operands and needs no move.
+
+constexpr int kUnit = 32;               // keys
+constexpr int kUnitTile = kUnit * kCacheHeadDim;  // bytes of K or V of a unit
+constexpr int kStreamWarps = 8;
+constexpr int kStreamThreads = kStreamWarps * 32;
+constexpr int kMinUnits = kStreamWarps;  // of a CTA: one for each warp
+
+// Ring slot beside the codes: scales and pages of the unit's two 16-key slabs.
+struct alignas(16) SlotInfo {
+  float scale[4];  // key, value of slab 0, of slab 1
+  int page[2];     // -1: nothing to see
+};
+
+struct StreamArgs {
+  CacheAttnArgs a;
+  uint32_t* counters;  // one for each (sequence, kv head); null: no item is split
+  float* parts;        // [CTA][2][JoinFloats(join_rows)]
+  int join_rows;       // rows of a (sequence, kv head) at most
+};
+
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                          uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9},"
+      " {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// Bytes 2i, 2i + 1 (kSel 0x4140, 0x4342) of four codes offset by 128, as
+// halves: 0x6400 | u is 1024 + u, less 1152 the code, all exact.
+template <uint32_t kSel>
+__device__ __forceinline__ uint32_t CodePair(uint32_t offset_codes) {
+  const uint32_t biased = __byte_perm(offset_codes, 0x64646464u, kSel);
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&biased),
+                            __half2half2(__ushort_as_half(0x6480)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+__device__ __forceinline__ void cp_async_4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src)
+               : "memory");
+}
+// Arrives on `bar` when this thread's cp.asyncs so far have landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+
+// Factor of a key scale in the exponent; a page of zeros has scale 0 and
+// scores 0, which any finite factor keeps.
+__device__ __forceinline__ float KeyFactor(float scale, float scale_log2) {
+  return scale == 0.0f ? 1.0f : scale * scale_log2;
+}
+// Units of a sequence and kv head; one (with nothing to see) where rows need
+// their zeros, none without rows.
+__device__ __forceinline__ int SequenceUnits(const CacheAttnArgs& a, int seq) {
+  const RowSpan span = SequenceRows(a.cu_rows, seq, a.rows, a.max_rows, a.err);
+  if (span.count == 0) return 0;
+  return max(1, (SequenceLength(a, seq) - 1) / kUnit + 1);
+}
+
+// One (sequence, kv head) among the numbered units.
+struct ItemAt {
+  int seq, head, units;
+  int64_t begin;  // its first unit's number
+  // To the next one that has units; false behind the last.
+  __device__ __forceinline__ bool Next(const CacheAttnArgs& a) {
+    begin += units;
+    if (++head < a.cache.kv_heads) return true;
+    head = 0;
+    while (++seq < a.cache.num_seqs) {
+      units = SequenceUnits(a, seq);
+      if (units > 0) return true;
+    }
+    return false;
+  }
+};
+
+struct alignas(16) StreamShared {
+  int64_t sum[kStreamWarps];
+  ItemAt first;
+  int last;
+};
+
+template <int kNT>
+constexpr int StreamStages() {
+  return kNT == 1 ? 3 : 2;
+}
+// Joining buffer of `rows` query rows: O, then maxima and sums, per warp.
+__host__ __device__ constexpr size_t JoinFloats(int rows) {
+  return (static_cast<size_t>(rows) * (kCacheHeadDim + 2) + 3) / 4 * 4;
+}
+template <int kNT>
+constexpr size_t StreamSmem(int rows) {
+  return 1024 + static_cast<size_t>(StreamStages<kNT>()) * kStreamWarps *
+                    (2 * kUnitTile + sizeof(SlotInfo) + sizeof(uint64_t)) +
+         sizeof(StreamShared) + kStreamWarps * JoinFloats(rows) * sizeof(float);
+}
+
+template <int kNT>
+__global__ void __launch_bounds__(kStreamThreads, 1)
+    cache_attention_stream_kernel(const __grid_constant__ CUtensorMap map_k,
+                                  const __grid_constant__ CUtensorMap map_v,
+                                  const StreamArgs args) {
+  constexpr int kStages = StreamStages<kNT>();
+  const CacheAttnArgs& a = args.a;
+  const CacheView& cache = a.cache;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int g = lane >> 2, c = lane & 3;
+  uint8_t* ring = smem + warp * (kStages * 2 * kUnitTile);
+  SlotInfo* info = reinterpret_cast<SlotInfo*>(smem + kStreamWarps * kStages * 2 * kUnitTile) +
+                   warp * kStages;
+  uint64_t* full = reinterpret_cast<uint64_t*>(
+                       smem + kStreamWarps * kStages * (2 * kUnitTile + sizeof(SlotInfo))) +
+                   warp * kStages;
+  StreamShared& shared = *reinterpret_cast<StreamShared*>(
+      smem + kStreamWarps * kStages * (2 * kUnitTile + sizeof(SlotInfo) + sizeof(uint64_t)));
+  float* join = reinterpret_cast<float*>(&shared + 1);
+  pdl_trigger();
+  if (lane == 0) {
+    // Lanes 0 and 1 each arrive for their codes and for their scales.
+    for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 4);
+    fence_mbar_init();
+    tma_prefetch_map(&map_k);
+    tma_prefetch_map(&map_v);
+  }
+  pdl_wait();
+
+  // This CTA's units [b0, b1) and the item that holds the first.
+  int64_t b0, b1, share = 0;
+  if (args.counters == nullptr) {
+    if (tid == 0) {
+      shared.first.seq = static_cast<int>(blockIdx.x) / cache.kv_heads;
+      shared.first.head = static_cast<int>(blockIdx.x) % cache.kv_heads;
+      shared.first.units = SequenceUnits(a, shared.first.seq);
+      shared.first.begin = 0;
+    }
+    __syncthreads();
+    b0 = 0;
+    b1 = shared.first.units;
+  } else {
+    const int per = (cache.num_seqs + kStreamThreads - 1) / kStreamThreads;
+    const int first = min(cache.num_seqs, tid * per), last = min(cache.num_seqs, first + per);
+    int64_t mine = 0;
+    for (int s = first; s < last; ++s) mine += SequenceUnits(a, s);
+    mine *= cache.kv_heads;
+    int64_t inclusive = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xFFFFFFFFu, inclusive, o);
+      if (lane >= o) inclusive += v;
+    }
+    if (lane == 31) shared.sum[warp] = inclusive;
+    __syncthreads();
+    int64_t total = 0, before = inclusive - mine;
+#pragma unroll
+    for (int w = 0; w < kStreamWarps; ++w) {
+      if (w < warp) before += shared.sum[w];
+      total += shared.sum[w];
+    }
+    share = max(static_cast<int64_t>(kMinUnits), (total + gridDim.x - 1) / gridDim.x);
+    b0 = share * blockIdx.x;
+    b1 = min(total, b0 + share);
+    if (before <= b0 && b0 < before + mine) {
+      for (int s = first; s < last; ++s) {
+        const int units = SequenceUnits(a, s);
+        const int64_t all = static_cast<int64_t>(units) * cache.kv_heads;
+        if (b0 < before + all) {
+          const int head = static_cast<int>((b0 - before) / units);
+          shared.first = {s, head, units, before + static_cast<int64_t>(head) * units};
+          break;
+        }
+        before += all;
+      }
+    }
+    __syncthreads();
+  }
+  if (b0 >= b1) return;
+  __syncwarp();
+
+  // The unit to load next (this warp's position q0) and its pages, one ahead.
+  ItemAt fetch = shared.first;
+  int64_t fetch_at = b0 + warp;
+  int fetch_page = -1;   // lanes 0 and 1: page of slab `lane`
+  int fetch_length = 0;
+  bool fetch_slot = false;  // whether this lane has a page to ask for
+  auto look_up = [&] {  // the page of this lane's slab of unit fetch_at
+    while (fetch_at < b1 && fetch_at >= fetch.begin + fetch.units) {
+      if (!fetch.Next(a)) break;
+    }
+    if (fetch_at >= b1) return;
+    fetch_length = SequenceLength(a, fetch.seq);
+    const int token = static_cast<int>(fetch_at - fetch.begin) * kUnit;
+    const int mine = token + (lane & 1) * 16;
+    fetch_slot = lane < 2 && mine < fetch_length;
+    if (fetch_slot)
+      fetch_page = cache.table[static_cast<int64_t>(fetch.seq) * cache.max_pages +
+                               (mine >> cache.page_shift)];
+  };
+  const int box = min(kUnit, 1 << cache.page_shift);  // rows of a TMA box
+  auto issue = [&](int stage) {
+    if (fetch_at >= b1) return;
+    if (lane < 2) {
+      uint64_t* bar = &full[stage];
+      int page = fetch_slot ? fetch_page : -1;
+      if (fetch_slot && (page < 0 || page >= cache.pages)) {
+        atomicOr(a.err, kErrBadArgument);
+        page = -1;
+      }
+      info[stage].page[lane] = page;
+      if (page >= 0) {
+        const int64_t at = static_cast<int64_t>(page) * cache.kv_heads + fetch.head;
+        cp_async_4(&info[stage].scale[2 * lane], cache.key_scales + at);
+        cp_async_4(&info[stage].scale[2 * lane + 1], cache.value_scales + at);
+      } else {
+        info[stage].scale[2 * lane] = info[stage].scale[2 * lane + 1] = 1.0f;
+      }
+      const bool loads = page >= 0 && (lane == 0 || box < kUnit);
+      if (loads) {
+        const int token = static_cast<int>(fetch_at - fetch.begin) * kUnit + lane * 16;
+        const int row = ((page * cache.kv_heads + fetch.head) << cache.page_shift) +
+                        (token & ((1 << cache.page_shift) - 1));
+        uint8_t* dst = ring + stage * 2 * kUnitTile + lane * 16 * kCacheHeadDim;
+        mbar_arrive_expect_tx(bar, 2 * box * kCacheHeadDim);
+        tma_load_2d(dst, &map_k, bar, 0, row);
+        tma_load_2d(dst + kUnitTile, &map_v, bar, 0, row);
+      } else {
+        mbar_arrive(bar);
+      }
+      cp_async_arrive(bar);
+    }
+    fetch_at += kStreamWarps;
+    look_up();
+  };
+  look_up();
+  for (int i = 0; i < kStages; ++i) issue(i);
+
+  // kappa(g) and kappa(2c), see above.
+  const int key_g = ((g & 1) << 2) | (g & 2) | (g >> 2);
+  const int key_c = ((c & 1) << 1) | (c >> 1);
+  // Lanes of c >= 2 read the later key of a pair first.
+  const bool later = c >= 2;
+  const uint32_t pair_lo = later ? 0x1504u : 0x5140u, pair_hi = later ? 0x3726u : 0x7362u;
+  int k_at[2], v_at[2];  // byte offsets in a slab of this lane's first reads
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    k_at[j] = key_g * kCacheHeadDim + (((4 * j + c) ^ key_g) << 4);
+    const int key = key_c + (later != (j == 1) ? 4 : 0);
+    v_at[j] = key * kCacheHeadDim + ((g ^ key) << 4);
+  }
+
+  ItemAt item = shared.first;
+  int64_t at = b0 + warp;
+  int done = 0;  // units of this warp so far
+  while (true) {
+    const int64_t item_end = item.begin + item.units;
+    const int64_t end = min(b1, item_end);
+    const RowSpan span = SequenceRows(a.cu_rows, item.seq, a.rows, a.max_rows, a.err);
+    const int length = SequenceLength(a, item.seq);
+    const int rows = span.count * a.group;  // row r: token r / group, head r % group
+    float m[kNT][2], l[kNT][2], o[8][kNT][4];
+    int seen[kNT][2];  // tokens that column 2c + e sees
+    uint32_t q[2][4][kNT][2];
+    const int least = a.causal ? length - span.count + 1 : length;
+#pragma unroll
+    for (int t = 0; t < kNT; ++t) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        m[t][e] = -INFINITY;
+        l[t][e] = 0.0f;
+        const int r = t * 8 + 2 * c + e;
+        seen[t][e] = a.causal && r < rows ? least + r / a.group : length;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][t][e] = 0.0f;
+    }
+    if (at < end) {
+#pragma unroll
+      for (int t = 0; t < kNT; ++t) {
+        const int r = t * 8 + g;
+        const bool live = r < rows;
+        const __half* src = a.q;
+        if (live)
+          src += static_cast<int64_t>(span.first + r / a.group) * a.ld_q +
+                 (item.head * a.group + r % a.group) * kCacheHeadDim + 16 * c;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint4 x = make_uint4(0, 0, 0, 0), y = x;
+          if (live) {
+            x = *reinterpret_cast<const uint4*>(src + 64 * j);
+            y = *reinterpret_cast<const uint4*>(src + 64 * j + 8);
+          }
+          q[j][0][t][0] = x.x, q[j][0][t][1] = x.y;
+          q[j][1][t][0] = x.z, q[j][1][t][1] = x.w;
+          q[j][2][t][0] = y.x, q[j][2][t][1] = y.y;
+          q[j][3][t][0] = y.z, q[j][3][t][1] = y.w;
+        }
+      }
+    }
+    for (; at < end; at += kStreamWarps) {
+      const int stage = done % kStages;
+      (void)mbar_wait(&full[stage], static_cast<uint32_t>(done / kStages) & 1u, a.err);
+      __syncwarp();
+      const uint8_t* keys = ring + stage * 2 * kUnitTile;
+      const uint8_t* values = keys + kUnitTile;
+      const int token0 = static_cast<int>(at - item.begin) * kUnit;
+      float s[2][kNT][4], shift[2], inverse[2];
+      const float4 scales = *reinterpret_cast<const float4*>(info[stage].scale);
+      const int2 pages = *reinterpret_cast<const int2*>(info[stage].page);
+      const float factor[2] = {KeyFactor(scales.x, a.scale_log2), KeyFactor(scales.z, a.scale_log2)};
+      ValueScale(scales.y, &shift[0], &inverse[0]);
+      ValueScale(scales.w, &shift[1], &inverse[1]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int t = 0; t < kNT; ++t) s[h][t][0] = s[h][t][1] = s[h][t][2] = s[h][t][3] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint8_t* p = keys + h * 16 * kCacheHeadDim + k_at[j];
+          const uint4 x = *reinterpret_cast<const uint4*>(p);
+          const uint4 y = *reinterpret_cast<const uint4*>(p + 8 * kCacheHeadDim);
+          const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const uint32_t u = xs[r] ^ 0x80808080u, v = ys[r] ^ 0x80808080u;
+            const uint32_t f[4] = {CodePair<0x4140>(u), CodePair<0x4140>(v), CodePair<0x4342>(u),
+                                   CodePair<0x4342>(v)};
+#pragma unroll
+            for (int t = 0; t < kNT; ++t) mma_16816(s[h][t], f, q[j][r][t][0], q[j][r][t][1]);
+          }
+        }
+      }
+      // Exponents, then the maximum, raised only when one passes it by 2^8.
+      const bool partial = token0 + kUnit > least || pages.x < 0 || pages.y < 0;
+      bool grow = false;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int t = 0; t < kNT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float& v = s[h][t][e];
+            v = fmaf(v, factor[h], shift[h]);
+            if (partial) {
+              const int key = token0 + h * 16 + key_g + (e >> 1) * 8;
+              if (key >= seen[t][e & 1] || (h == 0 ? pages.x : pages.y) < 0) v = -INFINITY;
+            }
+            grow |= v > m[t][e & 1] + 8.0f;
+          }
+      if (__any_sync(0xFFFFFFFFu, grow)) {
+#pragma unroll
+        for (int t = 0; t < kNT; ++t)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float top = fmaxf(fmaxf(s[0][t][e], s[0][t][e + 2]), fmaxf(s[1][t][e], s[1][t][e + 2]));
+            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
+            if (top > m[t][e]) {
+              const float old = Exp2Approx(m[t][e] - top);
+              m[t][e] = top;
+              l[t][e] *= old;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                o[i][t][e] *= old;
+                o[i][t][e + 2] *= old;
+              }
+            }
+          }
+      }
+      uint32_t pb[2][kNT][2];
+#pragma unroll
+      for (int t = 0; t < kNT; ++t) {
+        const float m0 = m[t][0] == -INFINITY ? 0.0f : m[t][0];
+        const float m1 = m[t][1] == -INFINITY ? 0.0f : m[t][1];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float p0 = Exp2Approx(s[h][t][0] - m0), p1 = Exp2Approx(s[h][t][1] - m1);
+          const float p2 = Exp2Approx(s[h][t][2] - m0), p3 = Exp2Approx(s[h][t][3] - m1);
+          l[t][0] = fmaf(p0 + p2, inverse[h], l[t][0]);
+          l[t][1] = fmaf(p1 + p3, inverse[h], l[t][1]);
+          pb[h][t][0] = transpose_8x8(pack_half2(p0, p1));
+          pb[h][t][1] = transpose_8x8(pack_half2(p2, p3));
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint8_t* p = values + h * 16 * kCacheHeadDim;
+        const uint4 x0 = *reinterpret_cast<const uint4*>(p + v_at[0]);
+        const uint4 x1 = *reinterpret_cast<const uint4*>(p + v_at[1]);
+        const uint4 x2 = *reinterpret_cast<const uint4*>(p + v_at[0] + 8 * kCacheHeadDim);
+        const uint4 x3 = *reinterpret_cast<const uint4*>(p + v_at[1] + 8 * kCacheHeadDim);
+        const uint32_t w0[4] = {x0.x, x0.y, x0.z, x0.w}, w1[4] = {x1.x, x1.y, x1.z, x1.w};
+        const uint32_t w2[4] = {x2.x, x2.y, x2.z, x2.w}, w3[4] = {x3.x, x3.y, x3.z, x3.w};
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const uint32_t u0 = w0[r] ^ 0x80808080u, u1 = w1[r] ^ 0x80808080u;
+          const uint32_t u2 = w2[r] ^ 0x80808080u, u3 = w3[r] ^ 0x80808080u;
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {  // dims 16 g + 4 r + 2 b, and one more
+            const uint32_t sel = b == 0 ? pair_lo : pair_hi;
+            const uint32_t near = __byte_perm(u0, u1, sel), far = __byte_perm(u2, u3, sel);
+            const uint32_t f[4] = {CodePair<0x4140>(near), CodePair<0x4342>(near),
+                                   CodePair<0x4140>(far), CodePair<0x4342>(far)};
+#pragma unroll
+            for (int t = 0; t < kNT; ++t) mma_16816(o[2 * r + b][t], f, pb[h][t][0], pb[h][t][1]);
+          }
+        }
+      }
+      ++done;
+      __syncwarp();
+      issue(stage);
+    }
+
+    // Join the warps' parts: O[row][128], then (maximum, sum) of each row.
+    float* part = join + warp * JoinFloats(args.join_rows);
+#pragma unroll
+    for (int t = 0; t < kNT; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float sum = l[t][e];
+        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 4);
+        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 8);
+        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 16);
+        const int r = t * 8 + 2 * c + e;
+        if (r < rows) {
+          float4* dst = reinterpret_cast<float4*>(part + r * kCacheHeadDim + 16 * g);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            dst[i] = make_float4(o[2 * i][t][e], o[2 * i][t][e + 2], o[2 * i + 1][t][e],
+                                 o[2 * i + 1][t][e + 2]);
+          if (g == 0) {
+            part[args.join_rows * kCacheHeadDim + 2 * r] = m[t][e];
+            part[args.join_rows * kCacheHeadDim + 2 * r + 1] = sum;
+          }
+        }
+      }
+    __syncthreads();
+    const bool whole = item.begin >= b0 && item_end <= b1;
+    const int stats = args.join_rows * kCacheHeadDim;
+    auto store_row = [&](int r, int d, float4 v, float sum) {
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      __half* dst = a.out + static_cast<int64_t>(span.first + r / a.group) * a.ld_out +
+                    (item.head * a.group + r % a.group) * kCacheHeadDim + d;
+      *reinterpret_cast<uint2*>(dst) =
+          make_uint2(pack_half2(v.x * inv, v.y * inv), pack_half2(v.z * inv, v.w * inv));
+    };
+    float* slot = whole ? nullptr
+                        : args.parts + (static_cast<int64_t>(blockIdx.x) * 2 +
+                                        (item.begin < b0 ? 0 : 1)) *
+                                           JoinFloats(args.join_rows);
+    for (int i = tid; i < rows * (kCacheHeadDim / 4); i += kStreamThreads) {
+      const int r = i / (kCacheHeadDim / 4), d = i % (kCacheHeadDim / 4) * 4;
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kStreamWarps; ++w)
+        top = fmaxf(top, join[w * JoinFloats(args.join_rows) + stats + 2 * r]);
+      const float base = top == -INFINITY ? 0.0f : top;
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      float sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kStreamWarps; ++w) {
+        const float* p = join + w * JoinFloats(args.join_rows);
+        const float f = Exp2Approx(p[stats + 2 * r] - base);
+        const float4 x = *reinterpret_cast<const float4*>(p + r * kCacheHeadDim + d);
+        v.x = fmaf(x.x, f, v.x);
+        v.y = fmaf(x.y, f, v.y);
+        v.z = fmaf(x.z, f, v.z);
+        v.w = fmaf(x.w, f, v.w);
+        sum = fmaf(p[stats + 2 * r + 1], f, sum);
+      }
+      if (whole) {
+        store_row(r, d, v, sum);
+      } else {
+        *reinterpret_cast<float4*>(slot + r * kCacheHeadDim + d) = v;
+        if (d == 0) *reinterpret_cast<float2*>(slot + stats + 2 * r) = make_float2(top, sum);
+        __threadfence();
+      }
+    }
+    __syncthreads();
+    if (!whole) {
+      // The last CTA of the item to arrive joins its parts, in CTA order.
+      const int first = static_cast<int>(item.begin / share);
+      const int last = static_cast<int>((item_end - 1) / share);
+      uint32_t* counter = args.counters + static_cast<int64_t>(item.seq) * cache.kv_heads + item.head;
+      if (tid == 0) {
+        __threadfence();
+        shared.last = atomicAdd(counter, 1u) == static_cast<uint32_t>(last - first);
+        if (shared.last) *counter = 0;
+      }
+      __syncthreads();
+      if (shared.last) {
+        __threadfence();
+        for (int i = tid; i < rows * (kCacheHeadDim / 4); i += kStreamThreads) {
+          const int r = i / (kCacheHeadDim / 4), d = i % (kCacheHeadDim / 4) * 4;
+          float top = -INFINITY, sum = 0.0f;
+          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+          for (int x = first; x <= last; ++x) {
+            const float* p = args.parts + (static_cast<int64_t>(x) * 2 +
+                                           (item.begin < x * share ? 0 : 1)) *
+                                              JoinFloats(args.join_rows);
+            const float2 ms = __ldcg(reinterpret_cast<const float2*>(p + stats + 2 * r));
+            const float4 y = __ldcg(reinterpret_cast<const float4*>(p + r * kCacheHeadDim + d));
+            const float grown = fmaxf(top, ms.x);
+            const float base = grown == -INFINITY ? 0.0f : grown;
+            const float f = Exp2Approx(top - base), h = Exp2Approx(ms.x - base);
+            v.x = fmaf(y.x, h, v.x * f);
+            v.y = fmaf(y.y, h, v.y * f);
+            v.z = fmaf(y.z, h, v.z * f);
+            v.w = fmaf(y.w, h, v.w * f);
+            sum = fmaf(ms.y, h, sum * f);
+            top = grown;
+          }
+          store_row(r, d, v, sum);
+        }
+      }
+      __syncthreads();
+    }
+    if (item_end >= b1 || !item.Next(a)) break;
+  }
+}
+
+// How a call runs: the streaming kernel's rows for a (sequence, kv head), its
+// CTAs and the scratch that splitting takes.
+struct StreamPlan {
+  int rows;       // 0: too many for it
+  unsigned ctas;
+  size_t counter_bytes, part_bytes;
+};
+
+StreamPlan PlanStream(const ov_kv_cache* cache, size_t max_rows, size_t max_length, size_t heads) {
+  StreamPlan plan{};
+  const size_t rows = max_rows * (heads / cache->kv_heads);
+  if (rows > 16) return plan;
+  plan.rows = static_cast<int>(rows);
+  const size_t items = cache->num_seqs * cache->kv_heads;
+  const size_t units = items * std::max<size_t>(1, (max_length + kUnit - 1) / kUnit);
+  plan.ctas = static_cast<unsigned>(
+      std::min<size_t>(SmCount(), (units + kMinUnits - 1) / kMinUnits));
+  plan.counter_bytes = (items * sizeof(uint32_t) + 15) / 16 * 16;
+  plan.part_bytes = 2 * plan.ctas * JoinFloats(plan.rows) * sizeof(float);
+  return plan;
+}
+
+template <int kNT>
+void LaunchStream(const StreamArgs& args, unsigned ctas, const CUtensorMap& map_k,
+                  const CUtensorMap& map_v, cudaStream_t stream) {
+  SetMaxDynamicSmem(reinterpret_cast<const void*>(cache_attention_stream_kernel<kNT>),
+                    static_cast<int>(StreamSmem<kNT>(8 * kNT)));
+  Launch(cache_attention_stream_kernel<kNT>, dim3(ctas), dim3(kStreamThreads),
+         StreamSmem<kNT>(args.join_rows), stream, "cache attention kernel launch", map_k, map_v,
+         args);
+}
+
+// A cache's codes as 128-byte rows, boxes of `box_rows` of them.
+void EncodeCodesMap(CUtensorMap* map, const int8_t* codes, const ov_kv_cache* cache,
+                    size_t box_rows, CUtensorMapSwizzle swizzle) {
+  EncodeTensorMap2D(map, codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, kCacheHeadDim,
+                    cache->pages * cache->kv_heads * cache->page_tokens, kCacheHeadDim,
+                    kCacheHeadDim, static_cast<uint32_t>(box_rows), swizzle);
+}
+
 }  // namespace
 }  // namespace ovb
 
@@ -114,8 +727,13 @@ extern "C" {
 
 size_t ov_attention_kv_cache_workspace_bytes(const ov_kv_cache* cache, size_t rows,
                                              size_t max_rows, size_t max_length, size_t heads) {
-  (void)cache, (void)rows, (void)max_rows, (void)max_length, (void)heads;
-  return 0;
+  size_t bytes = 0;
+  const int status = Guard("ov_attention_kv_cache_workspace_bytes: ", [&] {
+    OV_REQUIRE(cache != nullptr && cache->kv_heads > 0 && heads % cache->kv_heads == 0, "heads");
+    const StreamPlan plan = PlanStream(cache, std::min(max_rows, rows), max_length, heads);
+    if (plan.rows > 0) bytes = plan.counter_bytes + plan.part_bytes;
+  });
+  return status == OV_OK ? bytes : 0;
 }
 
 int ov_attention_kv_cache(const ov_kv_cache* cache, const uint16_t* q, size_t ld_q, size_t rows,
@@ -124,7 +742,6 @@ int ov_attention_kv_cache(const ov_kv_cache* cache, const uint16_t* q, size_t ld
                           size_t ld_out, void* workspace, size_t workspace_bytes,
                           ov_stream_t stream) {
   return Guard("ov_attention_kv_cache: ", [&] {
-    (void)workspace_bytes;
     const CacheView c = ViewCache(cache);
     OV_REQUIRE(heads > 0 && heads % cache->kv_heads == 0, "heads must be a multiple of kv_heads");
     OV_REQUIRE(heads <= 1024, "more than 1024 heads");
@@ -162,6 +779,23 @@ int ov_attention_kv_cache(const ov_kv_cache* cache, const uint16_t* q, size_t ld
     a.causal = causal != 0;
     a.scale_log2 = scale * 1.4426950408889634f;
     a.err = DeviceErrorWord();
+    const StreamPlan plan = PlanStream(cache, a.max_rows, max_length, heads);
+    if (plan.rows > 0) {
+      const size_t box = std::min<size_t>(kUnit, cache->page_tokens);
+      CUtensorMap map_k, map_v;
+      EncodeCodesMap(&map_k, c.keys, cache, box, CU_TENSOR_MAP_SWIZZLE_128B);
+      EncodeCodesMap(&map_v, c.values, cache, box, CU_TENSOR_MAP_SWIZZLE_128B);
+      StreamArgs args{a, nullptr, nullptr, plan.rows};
+      unsigned ctas = static_cast<unsigned>(c.num_seqs * c.kv_heads);
+      if (workspace != nullptr && workspace_bytes >= plan.counter_bytes + plan.part_bytes) {
+        args.counters = static_cast<uint32_t*>(workspace);
+        args.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.counter_bytes);
+        ctas = plan.ctas;
+      }
+      if (plan.rows <= 8) LaunchStream<1>(args, ctas, map_k, map_v, AsStream(stream));
+      else LaunchStream<2>(args, ctas, map_k, map_v, AsStream(stream));
+      return;
+    }
     const dim3 grid(static_cast<unsigned>((a.max_rows + 3) / 4), static_cast<unsigned>(c.num_seqs),
                     static_cast<unsigned>(heads));
     Launch(cache_attention_row_kernel, grid, dim3(128), 0, AsStream(stream),
