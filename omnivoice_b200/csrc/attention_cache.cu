@@ -16,6 +16,7 @@
 #include <cmath>
 #include <cstdint>
 
+#include "attention_device.cuh"
 #include "internal.hpp"
 #include "kv_cache.hpp"
 #include "launch.hpp"
@@ -57,12 +58,6 @@ __device__ __forceinline__ void ValueScale(float scale, float* shift, float* inv
   *inverse = b == b ? __fdividef(1.0f, b) : 0.0f;
 }
 
-__device__ __forceinline__ float Exp2Approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // Tokens of a sequence, bounded by what the call announced.
 __device__ __forceinline__ int SequenceLength(const CacheAttnArgs& a, int seq) {
   const int length = a.lengths[seq];
@@ -71,54 +66,6 @@ __device__ __forceinline__ int SequenceLength(const CacheAttnArgs& a, int seq) {
     return length < 0 ? 0 : a.max_length;
   }
   return length;
-}
-
-// One warp per (row, head): lane l holds head dimensions 4l .. 4l + 3, one
-// token after the other.
-__global__ void __launch_bounds__(128) cache_attention_row_kernel(const CacheAttnArgs a) {
-  pdl_trigger();
-  pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int head = blockIdx.z;
-  const int kv_head = head / a.group;
-  const int seq = blockIdx.y;
-  const RowSpan span = SequenceRows(a.cu_rows, seq, a.rows, a.max_rows, a.err);
-  const int i = static_cast<int>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (i >= span.count) return;
-  const int length = SequenceLength(a, seq);
-  const int seen = a.causal ? max(0, length - span.count + i + 1) : length;
-  const int64_t row = span.first + i;
-  const uint2 qp = *reinterpret_cast<const uint2*>(a.q + row * a.ld_q + head * kCacheHeadDim + lane * 4);
-  const float2 q0 = __half22float2(*reinterpret_cast<const __half2*>(&qp.x));
-  const float2 q1 = __half22float2(*reinterpret_cast<const __half2*>(&qp.y));
-  float m = -INFINITY, l = 0.0f, o[4] = {};
-  const int page_tokens = 1 << a.cache.page_shift;
-  for (int first = 0; first < seen; first += page_tokens) {
-    const int page = CachePage(a.cache, seq, first >> a.cache.page_shift, a.err);
-    if (page < 0) continue;
-    const int64_t at = static_cast<int64_t>(page) * a.cache.kv_heads + kv_head;
-    const float c = a.scale_log2 * a.cache.key_scales[at];
-    float shift, inverse;
-    ValueScale(a.cache.value_scales[at], &shift, &inverse);
-    const int64_t tile = CacheTile(a.cache, page, kv_head) + lane * 4;
-    const int n = min(page_tokens, seen - first);
-    for (int j = 0; j < n; ++j) {
-      const char4 kc = *reinterpret_cast<const char4*>(a.cache.keys + tile + j * kCacheHeadDim);
-      const char4 vc = *reinterpret_cast<const char4*>(a.cache.values + tile + j * kCacheHeadDim);
-      const float t = fmaf(warp_sum(q0.x * kc.x + q0.y * kc.y + q1.x * kc.z + q1.y * kc.w), c, shift);
-      const float top = fmaxf(m, t);
-      const float old = exp2f(m - top), p = exp2f(t - top);
-      m = top;
-      l = l * old + p * inverse;
-      o[0] = o[0] * old + p * vc.x;
-      o[1] = o[1] * old + p * vc.y;
-      o[2] = o[2] * old + p * vc.z;
-      o[3] = o[3] * old + p * vc.w;
-    }
-  }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  *reinterpret_cast<uint2*>(a.out + row * a.ld_out + head * kCacheHeadDim + lane * 4) =
-      make_uint2(pack_half2(o[0] * inv, o[1] * inv), pack_half2(o[2] * inv, o[3] * inv));
 }
 
 // ------------------------------------------- few rows: keys streamed by warps
@@ -203,6 +150,19 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
 __device__ __forceinline__ float KeyFactor(float scale, float scale_log2) {
   return scale == 0.0f ? 1.0f : scale * scale_log2;
 }
+// Adds a part (maximum and sum in ms, O in y) to a row's join.
+__device__ __forceinline__ void JoinPart(float* top, float* sum, float4* v, float2 ms, float4 y) {
+  const float grown = fmaxf(*top, ms.x);
+  const float base = grown == -INFINITY ? 0.0f : grown;
+  const float f = ex2_approx(*top - base), h = ex2_approx(ms.x - base);
+  v->x = fmaf(y.x, h, v->x * f);
+  v->y = fmaf(y.y, h, v->y * f);
+  v->z = fmaf(y.z, h, v->z * f);
+  v->w = fmaf(y.w, h, v->w * f);
+  *sum = fmaf(ms.y, h, *sum * f);
+  *top = grown;
+}
+
 // Units of a sequence and kv head; one (with nothing to see) where rows need
 // their zeros, none without rows.
 __device__ __forceinline__ int SequenceUnits(const CacheAttnArgs& a, int seq) {
@@ -407,6 +367,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
   ItemAt item = shared.first;
   int64_t at = b0 + warp;
   int done = 0;  // units of this warp so far
+  bool ok = true;  // once a wait ran out, no other is begun
   while (true) {
     const int64_t item_end = item.begin + item.units;
     const int64_t end = min(b1, item_end);
@@ -456,7 +417,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     }
     for (; at < end; at += kStreamWarps) {
       const int stage = done % kStages;
-      (void)mbar_wait(&full[stage], static_cast<uint32_t>(done / kStages) & 1u, a.err);
+      ok = ok && mbar_wait(&full[stage], static_cast<uint32_t>(done / kStages) & 1u, a.err);
       __syncwarp();
       const uint8_t* keys = ring + stage * 2 * kUnitTile;
       const uint8_t* values = keys + kUnitTile;
@@ -514,7 +475,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
             top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
             top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
             if (top > m[t][e]) {
-              const float old = Exp2Approx(m[t][e] - top);
+              const float old = ex2_approx(m[t][e] - top);
               m[t][e] = top;
               l[t][e] *= old;
 #pragma unroll
@@ -532,8 +493,8 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
         const float m1 = m[t][1] == -INFINITY ? 0.0f : m[t][1];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float p0 = Exp2Approx(s[h][t][0] - m0), p1 = Exp2Approx(s[h][t][1] - m1);
-          const float p2 = Exp2Approx(s[h][t][2] - m0), p3 = Exp2Approx(s[h][t][3] - m1);
+          const float p0 = ex2_approx(s[h][t][0] - m0), p1 = ex2_approx(s[h][t][1] - m1);
+          const float p2 = ex2_approx(s[h][t][2] - m0), p3 = ex2_approx(s[h][t][3] - m1);
           l[t][0] = fmaf(p0 + p2, inverse[h], l[t][0]);
           l[t][1] = fmaf(p1 + p3, inverse[h], l[t][1]);
           pb[h][t][0] = transpose_8x8(pack_half2(p0, p1));
@@ -618,7 +579,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
 #pragma unroll
       for (int w = 0; w < kStreamWarps; ++w) {
         const float* p = join + w * JoinFloats(args.join_rows);
-        const float f = Exp2Approx(p[stats + 2 * r] - base);
+        const float f = ex2_approx(p[stats + 2 * r] - base);
         const float4 x = *reinterpret_cast<const float4*>(p + r * kCacheHeadDim + d);
         v.x = fmaf(x.x, f, v.x);
         v.y = fmaf(x.y, f, v.y);
@@ -659,15 +620,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
                                               JoinFloats(args.join_rows);
             const float2 ms = __ldcg(reinterpret_cast<const float2*>(p + stats + 2 * r));
             const float4 y = __ldcg(reinterpret_cast<const float4*>(p + r * kCacheHeadDim + d));
-            const float grown = fmaxf(top, ms.x);
-            const float base = grown == -INFINITY ? 0.0f : grown;
-            const float f = Exp2Approx(top - base), h = Exp2Approx(ms.x - base);
-            v.x = fmaf(y.x, h, v.x * f);
-            v.y = fmaf(y.y, h, v.y * f);
-            v.z = fmaf(y.z, h, v.z * f);
-            v.w = fmaf(y.w, h, v.w * f);
-            sum = fmaf(ms.y, h, sum * f);
-            top = grown;
+            JoinPart(&top, &sum, &v, ms, y);
           }
           store_row(r, d, v, sum);
         }
@@ -675,6 +628,540 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
       __syncthreads();
     }
     if (item_end >= b1 || !item.Next(a)) break;
+  }
+}
+// ---------------------------------------- many rows: tiles on tcgen05
+//
+// The rows of a kv head (row r: token r / group, head r % group) in tiles of
+// 128, with attention_device.cuh's schedule: S = Q K^T into tensor memory,
+// the softmax's P written over it as half, O += P V.  What differs is how K
+// and V arrive: a warp loads their codes by TMA (32 KB for 128 keys instead
+// of 64), a converter warpgroup writes them as half into the swizzled tiles
+// that the MMAs read, once for two row tiles.  Two forms of a CTA:
+//   pairs   more than 128 rows: two tiles, one per softmax warpgroup, that
+//           share every K and V tile;
+//   single  up to 128 rows: both warpgroups take the same tile, one the even
+//           and one the odd key tiles, and join at the end.
+// Bound per key tile by the MMAs and the softmax's exponentials as in
+// ov_attention_varlen; the conversion (184 issue slots for each of its four
+// warps and tile) and the loads run beside them.
+//
+// Softmax registers: a CTA of 512 threads has 128 each, so scores are read
+// from tensor memory twice (maximum, then probabilities), 64 at a time,
+// instead of being held.
+
+constexpr int kSlabs = kKeys / 16;  // 16-key groups of a key tile: one page each at least
+constexpr int kScaleSlots = 8;
+constexpr int kMinKeyTiles = 2;  // of a split
+constexpr uint32_t kCodeTile = kKeys * kCacheHeadDim;  // 16 KB
+constexpr int kTileThreads = 512;
+constexpr int kConvertWarp = 8, kLoadWarp = 12, kMmaWarp = 13;
+
+// A slab's factor, shift and inverse value scale (ValueScale); bad: 1 where
+// its page does not exist.
+struct alignas(16) SlabScale {
+  float factor, shift, inverse;
+  int bad;
+};
+
+struct TileShared {
+  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2];
+  uint64_t codes_full[2], codes_empty[2];  // of keys, of values
+  uint64_t scale_full[kScaleSlots];
+  uint32_t tmem;
+  int last;
+  alignas(16) SlabScale scales[kScaleSlots][kSlabs];
+};
+
+constexpr size_t kTileSmem = 1024 + 6 * kTile + 2 * kCodeTile + sizeof(TileShared);
+// One part of a split item: O[row][128], then (maximum, sum) of its rows.
+__host__ __device__ constexpr size_t TilePartFloats(int tile_rows) {
+  return static_cast<size_t>(tile_rows) * (kCacheHeadDim + 2);
+}
+static_assert(kTileSmem <= 232448, "shared memory of a CTA");
+
+struct TileArgs {
+  CacheAttnArgs a;
+  uint32_t* counters;  // one for each (row tile of this grid, sequence, kv head)
+  float* parts;        // [counter][split]
+  int tile_rows;       // rows of a CTA: 128 or 256
+  int tiles;           // CTAs along the rows
+  int splits;          // CTAs along the keys, at most
+};
+
+__device__ __forceinline__ float Max16(const uint32_t* r) {
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = fmaxf(__uint_as_float(r[j]), __uint_as_float(r[j + 8]));
+#pragma unroll
+  for (int w = 4; w > 0; w >>= 1)
+#pragma unroll
+    for (int j = 0; j < w; ++j) v[j] = fmaxf(v[j], v[j + w]);
+  return v[0];
+}
+
+// Codes of 128 keys to a swizzled half tile ([2 boxes][128][64]), by 128 threads.
+// Rows of even and odd parity go through their two halves in opposite order,
+// so that 8 neighbouring lanes read and write all banks.
+__device__ __forceinline__ void ConvertTile(const uint8_t* codes, uint8_t* tile, int tid) {
+  const int part = tid & 3;
+#pragma unroll 4
+  for (int i = 0; i < 8; ++i) {
+    const int row = (i >> 1) * 32 + (tid >> 2);
+    const int box = (i & 1) ^ (row & 1);
+    const uint4 q = *reinterpret_cast<const uint4*>(codes + row * kCacheHeadDim + box * 64 + part * 16);
+    const uint32_t x = q.x ^ 0x80808080u, y = q.y ^ 0x80808080u;
+    const uint32_t z = q.z ^ 0x80808080u, w = q.w ^ 0x80808080u;
+    uint8_t* dst = tile + box * kHalfTile + row * 128;
+    *reinterpret_cast<uint4*>(dst + (((2 * part) ^ (row & 7)) << 4)) =
+        make_uint4(CodePair<0x4140>(x), CodePair<0x4342>(x), CodePair<0x4140>(y), CodePair<0x4342>(y));
+    *reinterpret_cast<uint4*>(dst + (((2 * part + 1) ^ (row & 7)) << 4)) =
+        make_uint4(CodePair<0x4140>(z), CodePair<0x4342>(z), CodePair<0x4140>(w), CodePair<0x4342>(w));
+  }
+}
+
+// MMA thread of the single form: key tile t belongs to group t & 1.
+__device__ __forceinline__ void IssueSingle(uint32_t tmem, const AttnBars& bars, uint8_t* q_s,
+                                            uint8_t* k_s, uint8_t* v_s, int nt, uint32_t* err) {
+  constexpr uint32_t idesc_s = idesc_f16_f32(kQ, kKeys, 0);
+  constexpr uint32_t idesc_o = idesc_f16_f32(kQ, kD, 1);
+  const uint32_t qa = smem_u32(q_s);
+  if (!mbar_wait(bars.q_full, 0, err)) return;
+  auto scores = [&](int t) {
+    const int g = t & 1;
+    if (!mbar_wait(&bars.k_full[g], static_cast<uint32_t>(t >> 1) & 1u, err)) return false;
+    tc_fence_after_sync();
+    const uint32_t ka = smem_u32(k_s + g * kTile);
+#pragma unroll
+    for (int kk = 0; kk < kD / 16; ++kk) {
+      const uint32_t off = (kk >> 2) * kHalfTile + (kk & 3) * 32;
+      umma_f16_ss(tmem + static_cast<uint32_t>(g * 256), smem_desc_sw128(qa + off, 16, 1024),
+                  smem_desc_sw128(ka + off, 16, 1024), idesc_s, kk > 0 ? 1u : 0u);
+    }
+    umma_commit(&bars.s_full[g]);
+    umma_commit(&bars.k_empty[g]);
+    return true;
+  };
+  for (int t = 0; t < min(2, nt); ++t)
+    if (!scores(t)) return;
+  for (int t = 0; t < nt; ++t) {
+    const int g = t & 1;
+    const uint32_t phase = static_cast<uint32_t>(t >> 1) & 1u;
+    if (!mbar_wait(&bars.p_full[g], phase, err) || !mbar_wait(&bars.v_full[g], phase, err)) return;
+    tc_fence_after_sync();
+    const uint32_t va = smem_u32(v_s + g * kTile);
+    const uint32_t p = tmem + static_cast<uint32_t>(g * 256);
+#pragma unroll
+    for (int kk = 0; kk < kKeys / 16; ++kk)
+      umma_f16_ts(p + 128, p + static_cast<uint32_t>(kk * 8),
+                  smem_desc_sw128(va + kk * 16 * 128, kHalfTile, 1024), idesc_o,
+                  (t > 1 || kk > 0) ? 1u : 0u);
+    umma_commit(&bars.v_empty[g]);
+    if (t + 2 >= nt) umma_commit(&bars.o_done[g]);
+    else if (!scores(t + 2)) return;
+  }
+}
+
+__global__ void __launch_bounds__(kTileThreads, 1)
+    cache_attention_tile_kernel(const __grid_constant__ CUtensorMap map_k,
+                                const __grid_constant__ CUtensorMap map_v, const TileArgs args) {
+  const CacheAttnArgs& a = args.a;
+  const CacheView& cache = a.cache;
+  pdl_trigger();
+  pdl_wait();
+  const int kv_head = blockIdx.z, seq = blockIdx.y;
+  // The last row tiles of a causal sequence see most: they start first.
+  const int tile = args.tiles - 1 - static_cast<int>(blockIdx.x) / args.splits;
+  const int split = static_cast<int>(blockIdx.x) % args.splits;
+  const RowSpan span = SequenceRows(a.cu_rows, seq, a.rows, a.max_rows, a.err);
+  const int rows = span.count * a.group;  // at most 2^31 (host check)
+  const int row0 = tile * args.tile_rows;
+  if (row0 >= rows) return;  // uniform over the CTA, before any barrier
+  const int length = SequenceLength(a, seq);
+  const bool pair = rows - row0 > kQ && args.tile_rows > kQ;
+  const int here = min(rows - row0, args.tile_rows);
+  const int last_token = (row0 + here - 1) / a.group;
+  const int reach = a.causal ? max(0, length - span.count + last_token + 1) : length;
+  const int all_tiles = (reach + kKeys - 1) / kKeys;
+  const int per = max(1, (all_tiles + args.splits - 1) / args.splits);
+  const int parts = max(1, (all_tiles + per - 1) / per);
+  if (split >= parts) return;
+  const int t0 = split * per;
+  const int nt = min(all_tiles, t0 + per) - t0;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint8_t* q_s = smem;               // [2 row tiles] x 32 KB
+  uint8_t* k_s = q_s + 2 * kTile;    // [2 stages] x 32 KB
+  uint8_t* v_s = k_s + 2 * kTile;    // [2 stages] x 32 KB
+  uint8_t* code_s = v_s + 2 * kTile; // keys, values: 16 KB each
+  TileShared& s = *reinterpret_cast<TileShared*>(code_s + 2 * kCodeTile);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  AttnBars bars;
+  bars.q_full = &s.q_full;
+  bars.k_full = s.k_full;
+  bars.k_empty = s.k_empty;
+  bars.v_full = s.v_full;
+  bars.v_empty = s.v_empty;
+  bars.s_full = s.s_full;
+  bars.p_full = s.p_full;
+  bars.o_done = s.o_done;
+  bars.pv_done = nullptr;
+  if (tid == 0) {
+    mbar_init(&s.q_full, 256);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.k_full[i], 128);
+      mbar_init(&s.v_full[i], 128);
+      mbar_init(&s.codes_full[i], kSlabs);
+      mbar_init(&s.codes_empty[i], 128);
+      mbar_init(&s.k_empty[i], 1);
+      mbar_init(&s.v_empty[i], 1);
+      mbar_init(&s.s_full[i], 1);
+      mbar_init(&s.p_full[i], 128);
+      mbar_init(&s.o_done[i], 1);
+    }
+    for (int i = 0; i < kScaleSlots; ++i) mbar_init(&s.scale_full[i], kSlabs);
+    fence_mbar_init();
+    tma_prefetch_map(&map_k);
+    tma_prefetch_map(&map_v);
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(&s.tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = s.tmem;
+  const int64_t item = (static_cast<int64_t>(tile) * cache.num_seqs + seq) * cache.kv_heads + kv_head;
+  float* part = parts > 1 ? args.parts + (item * args.splits + split) * TilePartFloats(args.tile_rows) : nullptr;
+  const int stats_at = args.tile_rows * kCacheHeadDim;
+
+  if (warp == kLoadWarp) {
+    // Lane i < 8 looks after slab i of a key tile; the first slab of a box
+    // loads it.  Codes wait for the converters, one key tile ahead of them.
+    const int box = min(kKeys, 1 << cache.page_shift);
+    auto look_up = [&](int t) {
+      const int token = (t0 + t) * kKeys + lane * 16;
+      return lane < kSlabs && t < nt && token < length
+                 ? cache.table[static_cast<int64_t>(seq) * cache.max_pages + (token >> cache.page_shift)]
+                 : -1;
+    };
+    int next = look_up(0);
+    for (int t = 0; t < nt; ++t) {
+      const int token = (t0 + t) * kKeys + lane * 16;
+      int page = next;
+      next = look_up(t + 1);
+      const bool wanted = token < length;
+      if (lane < kSlabs && wanted && (page < 0 || page >= cache.pages)) {
+        atomicOr(a.err, kErrBadArgument);
+        page = -1;
+      }
+      const int row = ((page * cache.kv_heads + kv_head) << cache.page_shift) +
+                      (token & ((1 << cache.page_shift) - 1));
+      bool ok = true;
+      for (int w = 0; w < 2 && ok; ++w) {
+        if (t > 0) ok = mbar_wait(&s.codes_empty[w], static_cast<uint32_t>(t - 1) & 1u, a.err);
+        if (lane < kSlabs) {
+          if (page >= 0 && lane * 16 % box == 0) {
+            mbar_arrive_expect_tx(&s.codes_full[w], box * kCacheHeadDim);
+            tma_load_2d(code_s + w * kCodeTile + lane * 16 * kCacheHeadDim, w == 0 ? &map_k : &map_v,
+                        &s.codes_full[w], 0, row);
+          } else {
+            mbar_arrive(&s.codes_full[w]);
+          }
+        }
+      }
+      if (lane < kSlabs) {
+        SlabScale v = {1.0f, 0.0f, 1.0f, wanted ? 1 : 0};
+        if (page >= 0) {
+          const int64_t at = static_cast<int64_t>(page) * cache.kv_heads + kv_head;
+          v.factor = KeyFactor(cache.key_scales[at], a.scale_log2);
+          ValueScale(cache.value_scales[at], &v.shift, &v.inverse);
+          v.bad = 0;
+        }
+        s.scales[t % kScaleSlots][lane] = v;
+        mbar_arrive(&s.scale_full[t % kScaleSlots]);
+      }
+      __syncwarp();
+      if (!__all_sync(0xFFFFFFFFu, ok)) break;
+    }
+  } else if (warp >= kConvertWarp && warp < kLoadWarp) {
+    const int ctid = tid - kConvertWarp * 32;
+    bool ok = true;  // once a wait ran out, no other is begun
+    for (int t = 0; t < nt; ++t) {
+      const int stage = t & 1;
+      const uint32_t reuse = static_cast<uint32_t>((t >> 1) - 1) & 1u;
+      ok = ok && mbar_wait(&s.codes_full[0], static_cast<uint32_t>(t) & 1u, a.err);
+      if (t >= 2) ok = ok && mbar_wait(&s.k_empty[stage], reuse, a.err);
+      ConvertTile(code_s, k_s + stage * kTile, ctid);
+      fence_proxy_async_smem();
+      mbar_arrive(&s.k_full[stage]);
+      mbar_arrive(&s.codes_empty[0]);
+      ok = ok && mbar_wait(&s.codes_full[1], static_cast<uint32_t>(t) & 1u, a.err);
+      if (t >= 2) ok = ok && mbar_wait(&s.v_empty[stage], reuse, a.err);
+      ConvertTile(code_s + kCodeTile, v_s + stage * kTile, ctid);
+      fence_proxy_async_smem();
+      mbar_arrive(&s.v_full[stage]);
+      mbar_arrive(&s.codes_empty[1]);
+    }
+  } else if (warp == kMmaWarp) {
+    if (lane == 0 && nt > 0) {
+      if (pair) {
+        AttnArgs issue{};
+        issue.err = a.err;
+        (void)AttnIssue(issue, tmem, bars, AttnPhase{}, q_s, k_s, v_s, 2, nt);
+      } else {
+        IssueSingle(tmem, bars, q_s, k_s, v_s, nt, a.err);
+      }
+    }
+  } else if (warp < kConvertWarp) {
+    // Query rows into the swizzled tiles, 16 lanes a row.
+    for (int r = tid >> 4; r < (pair ? 2 : 1) * kQ; r += 16) {
+      const int row = row0 + r, piece = tid & 15;
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (r < here)
+        x = *reinterpret_cast<const uint4*>(
+            a.q + static_cast<int64_t>(span.first + row / a.group) * a.ld_q +
+            (kv_head * a.group + row % a.group) * kCacheHeadDim + piece * 8);
+      *reinterpret_cast<uint4*>(q_s + (r >> 7) * kTile + (piece >> 3) * kHalfTile + (r & 127) * 128 +
+                                (((piece & 7) ^ (r & 7)) << 4)) = x;
+    }
+    fence_proxy_async_smem();
+    mbar_arrive(&s.q_full);
+
+    const int g = warp >> 2;
+    const int r = tid & 127;               // tensor-memory lane, row of the tile
+    const int mine = row0 + (pair ? g * kQ : 0) + r;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_addr = tmem + static_cast<uint32_t>(g * 256) + lanes;
+    const uint32_t o_addr = s_addr + 128;
+    const int before = length - span.count;  // tokens that row token 0 has before it
+    const int seen = a.causal ? min(length, before + mine / a.group + 1) : length;
+    // The fewest tokens that a row of this tile sees.
+    const int least = a.causal ? before + (mine - r) / a.group + 1 : length;
+    const int step = pair ? 1 : 2, first = pair ? 0 : g;
+    float m = -INFINITY, l = 0.0f;
+    int use = 0;
+    bool ok = true;
+    for (int t = first; t < nt; t += step, ++use) {
+      ok = ok && mbar_wait(&s.scale_full[t % kScaleSlots],
+                           static_cast<uint32_t>(t / kScaleSlots) & 1u, a.err);
+      const SlabScale* slab = s.scales[t % kScaleSlots];
+      ok = ok && mbar_wait(&s.s_full[g], static_cast<uint32_t>(use) & 1u, a.err);
+      __syncwarp();
+      tc_fence_after_sync();
+      const int token0 = (t0 + t) * kKeys;
+      int bad = 0;
+#pragma unroll
+      for (int i = 0; i < kSlabs; ++i) bad |= slab[i].bad;
+      const bool partial = token0 + kKeys > least || bad != 0;
+      const int valid = partial ? seen - token0 : kKeys;
+      float top = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t x[2][32];
+        tmem_ld_32x32b_x32(s_addr + c * 64, x[0]);
+        tmem_ld_32x32b_x32(s_addr + c * 64 + 32, x[1]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t* v = &x[i >> 1][(i & 1) * 16];
+          const SlabScale k = slab[c * 4 + i];
+          if (partial) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (c * 64 + i * 16 + j >= valid || k.bad) v[j] = 0xFF800000u;
+          }
+          top = fmaxf(top, fmaf(Max16(v), k.factor, k.shift));
+        }
+      }
+      bool rescale = false;
+      float alpha = 1.0f;
+      const bool grow = use == 0 ? top > m : top > m + kRescaleThreshold;
+      if (use == 0) {
+        m = top;
+      } else {
+        rescale = __any_sync(0xFFFFFFFFu, grow);
+        if (grow) {
+          alpha = ex2_approx(m - top);
+          m = top;
+        }
+      }
+      const float base = m == -INFINITY ? 0.0f : m;
+      float sum = 0.0f;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t x[2][32];
+        tmem_ld_32x32b_x32(s_addr + c * 64, x[0]);
+        tmem_ld_32x32b_x32(s_addr + c * 64 + 32, x[1]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t packed[16];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const SlabScale k = slab[c * 4 + h * 2 + i];
+            const float shift = k.shift - base;
+            float p0 = 0.0f, p1 = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) {
+              float e0 = fmaf(__uint_as_float(x[h][i * 16 + j]), k.factor, shift);
+              float e1 = fmaf(__uint_as_float(x[h][i * 16 + j + 1]), k.factor, shift);
+              if (partial) {
+                const int key = c * 64 + h * 32 + i * 16 + j;
+                if (key >= valid || k.bad) e0 = -INFINITY;
+                if (key + 1 >= valid || k.bad) e1 = -INFINITY;
+              }
+              e0 = ex2_approx(e0);
+              e1 = ex2_approx(e1);
+              p0 += e0;
+              p1 += e1;
+              packed[i * 8 + j / 2] = pack_half2(e0, e1);
+            }
+            sum = fmaf(p0 + p1, k.inverse, sum);
+          }
+          tmem_st_32x32b_x16(s_addr + c * 32 + h * 16, packed);
+        }
+      }
+      if (rescale) {
+        l *= alpha;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t x[32];
+          tmem_ld_32x32b_x32(o_addr + c * 32, x);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * alpha);
+          tmem_st_32x32b_x16(o_addr + c * 32, *reinterpret_cast<const uint32_t(*)[16]>(&x[0]));
+          tmem_st_32x32b_x16(o_addr + c * 32 + 16, *reinterpret_cast<const uint32_t(*)[16]>(&x[16]));
+        }
+      }
+      l += sum;
+      tmem_st_wait();
+      tc_fence_before_sync();
+      mbar_arrive(&s.p_full[g]);
+    }
+
+    // O of this warpgroup's tiles; in the single form the odd key tiles'
+    // half goes through shared memory (every MMA is done: the rings are idle).
+    const bool any = nt > first;
+    if (pair && any) ok = ok && mbar_wait(&s.o_done[g], 0, a.err);
+    if (!pair && nt > 0) ok = ok && mbar_wait(&s.o_done[0], 0, a.err);
+    if (!pair && nt > 1) ok = ok && mbar_wait(&s.o_done[1], 0, a.err);
+    __syncwarp();
+    tc_fence_after_sync();
+    constexpr int kPad = kCacheHeadDim + 4;
+    float* other = reinterpret_cast<float*>(k_s) + r * kPad;
+    float scale_mine = 1.0f, scale_other = 0.0f;
+    if (!pair) {
+      float2* stats = reinterpret_cast<float2*>(k_s + kQ * kPad * sizeof(float)) + r;
+      if (g == 1) {
+        if (any) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t x[32];
+            tmem_ld_32x32b_x32(o_addr + c * 32, x);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; j += 4)
+              *reinterpret_cast<uint4*>(other + c * 32 + j) = make_uint4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+          }
+        }
+        *stats = make_float2(m, l);
+      }
+      named_barrier(1, 256);
+      if (g == 0) {
+        const float2 o = *stats;
+        const float top = fmaxf(m, o.x);
+        const float base = top == -INFINITY ? 0.0f : top;
+        scale_mine = ex2_approx(m - base);
+        scale_other = ex2_approx(o.x - base);
+        l = l * scale_mine + o.y * scale_other;
+        m = top;
+      }
+    }
+    if (pair || g == 0) {
+      const bool store = mine - row0 < here;
+      const float inv = part != nullptr ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+      const int at = mine - row0;  // row of this CTA
+      __half* dst = a.out + static_cast<int64_t>(span.first + mine / a.group) * a.ld_out +
+                    (kv_head * a.group + mine % a.group) * kCacheHeadDim;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t x[32];
+        float o[32];
+        if (nt > 0) {
+          tmem_ld_32x32b_x32(o_addr + c * 32, x);
+          tmem_ld_wait();
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) o[j] = nt > 0 ? __uint_as_float(x[j]) * scale_mine : 0.0f;
+        if (!pair && nt > 1) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const float4 y = *reinterpret_cast<const float4*>(other + c * 32 + j);
+            o[j] = fmaf(y.x, scale_other, o[j]);
+            o[j + 1] = fmaf(y.y, scale_other, o[j + 1]);
+            o[j + 2] = fmaf(y.z, scale_other, o[j + 2]);
+            o[j + 3] = fmaf(y.w, scale_other, o[j + 3]);
+          }
+        }
+        if (!store) continue;
+        if (part != nullptr) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4)
+            *reinterpret_cast<float4*>(part + at * kCacheHeadDim + c * 32 + j) =
+                make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; j += 8)
+            *reinterpret_cast<uint4*>(dst + c * 32 + j) =
+                make_uint4(pack_half2(o[j] * inv, o[j + 1] * inv), pack_half2(o[j + 2] * inv, o[j + 3] * inv),
+                           pack_half2(o[j + 4] * inv, o[j + 5] * inv), pack_half2(o[j + 6] * inv, o[j + 7] * inv));
+        }
+      }
+      if (part != nullptr && store) {
+        *reinterpret_cast<float2*>(part + stats_at + 2 * at) = make_float2(m, l);
+        __threadfence();
+      }
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, 512);
+  }
+  if (part == nullptr) return;
+  // The last part to arrive joins all of them, in split order.
+  uint32_t* counter = args.counters + item;
+  if (tid == 0) {
+    __threadfence();
+    s.last = atomicAdd(counter, 1u) == static_cast<uint32_t>(parts - 1);
+    if (s.last) *counter = 0;
+  }
+  __syncthreads();
+  if (!s.last) return;
+  __threadfence();
+  const float* base_part = args.parts + item * args.splits * TilePartFloats(args.tile_rows);
+  for (int i = tid; i < here * (kCacheHeadDim / 4); i += kTileThreads) {
+    const int at = i / (kCacheHeadDim / 4), d = i % (kCacheHeadDim / 4) * 4;
+    float top = -INFINITY, sum = 0.0f;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int x = 0; x < parts; ++x) {
+      const float* p = base_part + x * TilePartFloats(args.tile_rows);
+      const float2 ms = __ldcg(reinterpret_cast<const float2*>(p + stats_at + 2 * at));
+      const float4 y = __ldcg(reinterpret_cast<const float4*>(p + at * kCacheHeadDim + d));
+      JoinPart(&top, &sum, &v, ms, y);
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int row = row0 + at;
+    *reinterpret_cast<uint2*>(a.out + static_cast<int64_t>(span.first + row / a.group) * a.ld_out +
+                              (kv_head * a.group + row % a.group) * kCacheHeadDim + d) =
+        make_uint2(pack_half2(v.x * inv, v.y * inv), pack_half2(v.z * inv, v.w * inv));
   }
 }
 
@@ -697,6 +1184,31 @@ StreamPlan PlanStream(const ov_kv_cache* cache, size_t max_rows, size_t max_leng
       std::min<size_t>(SmCount(), (units + kMinUnits - 1) / kMinUnits));
   plan.counter_bytes = (items * sizeof(uint32_t) + 15) / 16 * 16;
   plan.part_bytes = 2 * plan.ctas * JoinFloats(plan.rows) * sizeof(float);
+  return plan;
+}
+
+// The tile kernel's CTAs and scratch.
+struct TilePlan {
+  int tile_rows, tiles, splits;
+  size_t counter_bytes, part_bytes;
+};
+
+TilePlan PlanTiles(const ov_kv_cache* cache, size_t max_rows, size_t max_length, size_t heads) {
+  TilePlan plan{};
+  const size_t rows = max_rows * (heads / cache->kv_heads);
+  const size_t pairs = cache->num_seqs * cache->kv_heads;  // of sequence and kv head
+  const size_t sms = static_cast<size_t>(SmCount());
+  // Single tiles while they all fit the GPU at once, else tile pairs.
+  plan.tile_rows = (rows + kQ - 1) / kQ * pairs <= sms ? kQ : 2 * kQ;
+  plan.tiles = static_cast<int>((rows + plan.tile_rows - 1) / plan.tile_rows);
+  const size_t items = plan.tiles * pairs;
+  const size_t key_tiles = (max_length + kKeys - 1) / kKeys;
+  plan.splits = static_cast<int>(
+      std::max<size_t>(1, std::min(sms / items, key_tiles / kMinKeyTiles)));
+  if (plan.splits > 1) {
+    plan.counter_bytes = (items * sizeof(uint32_t) + 15) / 16 * 16;
+    plan.part_bytes = items * plan.splits * TilePartFloats(plan.tile_rows) * sizeof(float);
+  }
   return plan;
 }
 
@@ -729,9 +1241,16 @@ size_t ov_attention_kv_cache_workspace_bytes(const ov_kv_cache* cache, size_t ro
                                              size_t max_rows, size_t max_length, size_t heads) {
   size_t bytes = 0;
   const int status = Guard("ov_attention_kv_cache_workspace_bytes: ", [&] {
-    OV_REQUIRE(cache != nullptr && cache->kv_heads > 0 && heads % cache->kv_heads == 0, "heads");
+    OV_REQUIRE(cache != nullptr && cache->kv_heads > 0, "cache");
+    OV_REQUIRE(heads > 0 && heads % cache->kv_heads == 0, "heads must be a multiple of kv_heads");
+    if (std::min(max_rows, rows) == 0 || cache->num_seqs == 0) return;
     const StreamPlan plan = PlanStream(cache, std::min(max_rows, rows), max_length, heads);
-    if (plan.rows > 0) bytes = plan.counter_bytes + plan.part_bytes;
+    if (plan.rows > 0) {
+      bytes = plan.counter_bytes + plan.part_bytes;
+    } else {
+      const TilePlan tiles = PlanTiles(cache, std::min(max_rows, rows), max_length, heads);
+      bytes = tiles.counter_bytes + tiles.part_bytes;
+    }
   });
   return status == OV_OK ? bytes : 0;
 }
@@ -751,6 +1270,8 @@ int ov_attention_kv_cache(const ov_kv_cache* cache, const uint16_t* q, size_t ld
                "max_length exceeds the page table");
     OV_REQUIRE(ld_q % 8 == 0 && ld_q >= heads * kCacheHeadDim, "q stride");
     OV_REQUIRE(ld_out % 8 == 0 && ld_out >= heads * kCacheHeadDim, "out stride");
+    OV_REQUIRE(std::min(max_rows, rows) <= ((size_t{1} << 31) - 512) / (heads / cache->kv_heads),
+               "max_rows * heads / kv_heads must stay below 2^31");
     if (rows == 0 || max_rows == 0 || c.num_seqs == 0) return;
     RequireAligned(q, 16, "q");
     RequireAligned(out, 16, "out");
@@ -796,10 +1317,27 @@ int ov_attention_kv_cache(const ov_kv_cache* cache, const uint16_t* q, size_t ld
       else LaunchStream<2>(args, ctas, map_k, map_v, AsStream(stream));
       return;
     }
-    const dim3 grid(static_cast<unsigned>((a.max_rows + 3) / 4), static_cast<unsigned>(c.num_seqs),
-                    static_cast<unsigned>(heads));
-    Launch(cache_attention_row_kernel, grid, dim3(128), 0, AsStream(stream),
-           "cache attention kernel launch", a);
+    TilePlan tiles = PlanTiles(cache, a.max_rows, max_length, heads);
+    TileArgs args{a, nullptr, nullptr, tiles.tile_rows, tiles.tiles, tiles.splits};
+    if (tiles.splits > 1) {
+      if (workspace != nullptr && workspace_bytes >= tiles.counter_bytes + tiles.part_bytes) {
+        args.counters = static_cast<uint32_t*>(workspace);
+        args.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + tiles.counter_bytes);
+      } else {
+        args.splits = 1;
+      }
+    }
+    const size_t box = std::min<size_t>(kKeys, cache->page_tokens);
+    CUtensorMap map_k, map_v;
+    EncodeCodesMap(&map_k, c.keys, cache, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+    EncodeCodesMap(&map_v, c.values, cache, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+    SetMaxDynamicSmem(reinterpret_cast<const void*>(cache_attention_tile_kernel),
+                      static_cast<int>(kTileSmem));
+    Launch(cache_attention_tile_kernel,
+           dim3(static_cast<unsigned>(args.tiles) * static_cast<unsigned>(args.splits),
+                static_cast<unsigned>(c.num_seqs), static_cast<unsigned>(c.kv_heads)),
+           dim3(kTileThreads), kTileSmem, AsStream(stream), "cache attention kernel launch", map_k,
+           map_v, args);
   });
 }
 
