@@ -26,6 +26,20 @@
 namespace ovb {
 namespace {
 
+// Division of 0 <= n < 2^31 by d through a multiplication (Granlund &
+// Montgomery, "Division by invariant integers using multiplication", 1994).
+struct FastDiv {
+  int d;
+  uint32_t mul, shift;
+  explicit FastDiv(int divisor) : d(divisor), mul(0), shift(0) {
+    while ((1ll << shift) < d) ++shift;
+    mul = static_cast<uint32_t>((((1ull << shift) - d) << 32) / d + 1);
+  }
+  __device__ __forceinline__ int operator()(int n) const {
+    return static_cast<int>((__umulhi(static_cast<uint32_t>(n), mul) + n) >> shift);
+  }
+};
+
 struct CacheAttnArgs {
   CacheView cache;
   const __half* q;
@@ -38,7 +52,7 @@ struct CacheAttnArgs {
   int max_rows;
   int max_length;
   int heads;
-  int group;  // heads / kv_heads
+  FastDiv group;  // heads / kv_heads
   int causal;
   float scale_log2;  // softmax scale * log2(e)
   uint32_t* err;
@@ -150,17 +164,24 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
 __device__ __forceinline__ float KeyFactor(float scale, float scale_log2) {
   return scale == 0.0f ? 1.0f : scale * scale_log2;
 }
-// Adds a part (maximum and sum in ms, O in y) to a row's join.
-__device__ __forceinline__ void JoinPart(float* top, float* sum, float4* v, float2 ms, float4 y) {
+// Adds a part's maximum and sum (ms) to a row's; returns the factors of the
+// O so far and of the part's O.
+__device__ __forceinline__ float2 JoinFactors(float* top, float* sum, float2 ms) {
   const float grown = fmaxf(*top, ms.x);
   const float base = grown == -INFINITY ? 0.0f : grown;
   const float f = ex2_approx(*top - base), h = ex2_approx(ms.x - base);
+  *sum = fmaf(ms.y, h, *sum * f);
+  *top = grown;
+  return make_float2(f, h);
+}
+
+__device__ __forceinline__ void JoinPart(float* top, float* sum, float4* v, float2 ms, float4 y) {
+  const float2 factors = JoinFactors(top, sum, ms);
+  const float f = factors.x, h = factors.y;
   v->x = fmaf(y.x, h, v->x * f);
   v->y = fmaf(y.y, h, v->y * f);
   v->z = fmaf(y.z, h, v->z * f);
   v->w = fmaf(y.w, h, v->w * f);
-  *sum = fmaf(ms.y, h, *sum * f);
-  *top = grown;
 }
 
 // Units of a sequence and kv head; one (with nothing to see) where rows need
@@ -373,7 +394,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     const int64_t end = min(b1, item_end);
     const RowSpan span = SequenceRows(a.cu_rows, item.seq, a.rows, a.max_rows, a.err);
     const int length = SequenceLength(a, item.seq);
-    const int rows = span.count * a.group;  // row r: token r / group, head r % group
+    const int rows = span.count * a.group.d;  // row r: token r / group, head r % group
     float m[kNT][2], l[kNT][2], o[8][kNT][4];
     int seen[kNT][2];  // tokens that column 2c + e sees
     uint32_t q[2][4][kNT][2];
@@ -385,7 +406,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
         m[t][e] = -INFINITY;
         l[t][e] = 0.0f;
         const int r = t * 8 + 2 * c + e;
-        seen[t][e] = a.causal && r < rows ? least + r / a.group : length;
+        seen[t][e] = a.causal && r < rows ? least + a.group(r) : length;
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -398,9 +419,11 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
         const int r = t * 8 + g;
         const bool live = r < rows;
         const __half* src = a.q;
-        if (live)
-          src += static_cast<int64_t>(span.first + r / a.group) * a.ld_q +
-                 (item.head * a.group + r % a.group) * kCacheHeadDim + 16 * c;
+        if (live) {
+          const int token = a.group(r);
+          src += static_cast<int64_t>(span.first + token) * a.ld_q +
+                 (item.head * a.group.d + r - token * a.group.d) * kCacheHeadDim + 16 * c;
+        }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           uint4 x = make_uint4(0, 0, 0, 0), y = x;
@@ -558,8 +581,9 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     const int stats = args.join_rows * kCacheHeadDim;
     auto store_row = [&](int r, int d, float4 v, float sum) {
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      __half* dst = a.out + static_cast<int64_t>(span.first + r / a.group) * a.ld_out +
-                    (item.head * a.group + r % a.group) * kCacheHeadDim + d;
+      const int token = a.group(r);
+      __half* dst = a.out + static_cast<int64_t>(span.first + token) * a.ld_out +
+                    (item.head * a.group.d + r - token * a.group.d) * kCacheHeadDim + d;
       *reinterpret_cast<uint2*>(dst) =
           make_uint2(pack_half2(v.x * inv, v.y * inv), pack_half2(v.z * inv, v.w * inv));
     };
@@ -646,9 +670,8 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
 // ov_attention_varlen; the conversion (184 issue slots for each of its four
 // warps and tile) and the loads run beside them.
 //
-// Softmax registers: a CTA of 512 threads has 128 each, so scores are read
-// from tensor memory twice (maximum, then probabilities), 64 at a time,
-// instead of being held.
+// Registers: 512 threads start with 128 each; the softmax warpgroups, which
+// hold a row's 128 scores, take 184 and the other two keep 72.
 
 constexpr int kSlabs = kKeys / 16;  // 16-key groups of a key tile: one page each at least
 constexpr int kScaleSlots = 8;
@@ -674,7 +697,8 @@ struct TileShared {
 };
 
 constexpr size_t kTileSmem = 1024 + 6 * kTile + 2 * kCodeTile + sizeof(TileShared);
-// One part of a split item: O[row][128], then (maximum, sum) of its rows.
+// One part of a split item: O[32 vectors of 4 columns][row], then (maximum,
+// sum) of its rows.
 __host__ __device__ constexpr size_t TilePartFloats(int tile_rows) {
   return static_cast<size_t>(tile_rows) * (kCacheHeadDim + 2);
 }
@@ -700,65 +724,129 @@ __device__ __forceinline__ float Max16(const uint32_t* r) {
   return v[0];
 }
 
-// Codes of 128 keys to a swizzled half tile ([2 boxes][128][64]), by 128 threads.
-// Rows of even and odd parity go through their two halves in opposite order,
-// so that 8 neighbouring lanes read and write all banks.
+// 16 codes to 16 halves, in two 16-byte pieces.
+__device__ __forceinline__ void Convert16(const uint8_t* codes, uint8_t* low, uint8_t* high) {
+  const uint4 q = *reinterpret_cast<const uint4*>(codes);
+  const uint32_t x = q.x ^ 0x80808080u, y = q.y ^ 0x80808080u;
+  const uint32_t z = q.z ^ 0x80808080u, w = q.w ^ 0x80808080u;
+  *reinterpret_cast<uint4*>(low) =
+      make_uint4(CodePair<0x4140>(x), CodePair<0x4342>(x), CodePair<0x4140>(y), CodePair<0x4342>(y));
+  *reinterpret_cast<uint4*>(high) =
+      make_uint4(CodePair<0x4140>(z), CodePair<0x4342>(z), CodePair<0x4140>(w), CodePair<0x4342>(w));
+}
+
+// Codes of 128 keys to a swizzled half tile ([2 boxes][128][64]), by 128
+// threads: 16 codes of each 64-dim half of every 32nd row.  Even and odd rows
+// take their halves in opposite order, so that 8 neighbouring lanes read and
+// write all banks.
 __device__ __forceinline__ void ConvertTile(const uint8_t* codes, uint8_t* tile, int tid) {
-  const int part = tid & 3;
-#pragma unroll 4
-  for (int i = 0; i < 8; ++i) {
-    const int row = (i >> 1) * 32 + (tid >> 2);
-    const int box = (i & 1) ^ (row & 1);
-    const uint4 q = *reinterpret_cast<const uint4*>(codes + row * kCacheHeadDim + box * 64 + part * 16);
-    const uint32_t x = q.x ^ 0x80808080u, y = q.y ^ 0x80808080u;
-    const uint32_t z = q.z ^ 0x80808080u, w = q.w ^ 0x80808080u;
-    uint8_t* dst = tile + box * kHalfTile + row * 128;
-    *reinterpret_cast<uint4*>(dst + (((2 * part) ^ (row & 7)) << 4)) =
-        make_uint4(CodePair<0x4140>(x), CodePair<0x4342>(x), CodePair<0x4140>(y), CodePair<0x4342>(y));
-    *reinterpret_cast<uint4*>(dst + (((2 * part + 1) ^ (row & 7)) << 4)) =
-        make_uint4(CodePair<0x4140>(z), CodePair<0x4342>(z), CodePair<0x4140>(w), CodePair<0x4342>(w));
+  const int part = tid & 3, row = tid >> 2, box = row & 1;
+  const uint8_t* src = codes + row * kCacheHeadDim + part * 16;
+  uint8_t* low = tile + row * 128 + (((2 * part) ^ (row & 7)) << 4);
+  uint8_t* high = tile + row * 128 + (((2 * part + 1) ^ (row & 7)) << 4);
+  const uint32_t first = box * kHalfTile, second = kHalfTile - first;
+  const uint8_t* src_first = src + box * 64;
+  const uint8_t* src_second = src + 64 - box * 64;
+#pragma unroll 2
+  for (int i = 0; i < 4; ++i) {
+    Convert16(src_first + i * 32 * kCacheHeadDim, low + first + i * 32 * 128, high + first + i * 32 * 128);
+    Convert16(src_second + i * 32 * kCacheHeadDim, low + second + i * 32 * 128, high + second + i * 32 * 128);
   }
 }
 
-// MMA thread of the single form: key tile t belongs to group t & 1.
-__device__ __forceinline__ void IssueSingle(uint32_t tmem, const AttnBars& bars, uint8_t* q_s,
-                                            uint8_t* k_s, uint8_t* v_s, int nt, uint32_t* err) {
-  constexpr uint32_t idesc_s = idesc_f16_f32(kQ, kKeys, 0);
-  constexpr uint32_t idesc_o = idesc_f16_f32(kQ, kD, 1);
-  const uint32_t qa = smem_u32(q_s);
-  if (!mbar_wait(bars.q_full, 0, err)) return;
-  auto scores = [&](int t) {
-    const int g = t & 1;
-    if (!mbar_wait(&bars.k_full[g], static_cast<uint32_t>(t >> 1) & 1u, err)) return false;
-    tc_fence_after_sync();
-    const uint32_t ka = smem_u32(k_s + g * kTile);
+// The products of one CTA, issued by one thread.  A step along the head
+// dimension or the keys only adds to a descriptor's address field.
+struct TileIssue {
+  uint32_t tmem;
+  uint64_t q, k, v;  // descriptors of row tile 0 and of stage 0
+
+  __device__ __forceinline__ TileIssue(uint32_t tmem_, const uint8_t* q_s, const uint8_t* k_s,
+                                       const uint8_t* v_s)
+      : tmem(tmem_),
+        q(smem_desc_sw128(smem_u32(q_s), 16, 1024)),
+        k(smem_desc_sw128(smem_u32(k_s), 16, 1024)),
+        v(smem_desc_sw128(smem_u32(v_s), kHalfTile, 1024)) {}
+  // S of group g = Q of row tile `tile` x K of `stage`.
+  __device__ __forceinline__ void Scores(int g, int tile, int stage) const {
+    constexpr uint32_t idesc = idesc_f16_f32(kQ, kKeys, 0);
+    const uint64_t qd = q + static_cast<uint32_t>(tile) * (kTile >> 4);
+    const uint64_t kd = k + static_cast<uint32_t>(stage) * (kTile >> 4);
 #pragma unroll
     for (int kk = 0; kk < kD / 16; ++kk) {
-      const uint32_t off = (kk >> 2) * kHalfTile + (kk & 3) * 32;
-      umma_f16_ss(tmem + static_cast<uint32_t>(g * 256), smem_desc_sw128(qa + off, 16, 1024),
-                  smem_desc_sw128(ka + off, 16, 1024), idesc_s, kk > 0 ? 1u : 0u);
+      const uint32_t off = ((kk >> 2) * kHalfTile + (kk & 3) * 32) >> 4;
+      umma_f16_ss(tmem + static_cast<uint32_t>(g * 256), qd + off, kd + off, idesc, kk > 0 ? 1u : 0u);
     }
-    umma_commit(&bars.s_full[g]);
-    umma_commit(&bars.k_empty[g]);
-    return true;
-  };
-  for (int t = 0; t < min(2, nt); ++t)
-    if (!scores(t)) return;
-  for (int t = 0; t < nt; ++t) {
-    const int g = t & 1;
-    const uint32_t phase = static_cast<uint32_t>(t >> 1) & 1u;
-    if (!mbar_wait(&bars.p_full[g], phase, err) || !mbar_wait(&bars.v_full[g], phase, err)) return;
-    tc_fence_after_sync();
-    const uint32_t va = smem_u32(v_s + g * kTile);
+  }
+  // O of group g (+)= its P x V of `stage`.
+  __device__ __forceinline__ void Values(int g, int stage, bool add) const {
+    constexpr uint32_t idesc = idesc_f16_f32(kQ, kD, 1);
+    const uint64_t vd = v + static_cast<uint32_t>(stage) * (kTile >> 4);
     const uint32_t p = tmem + static_cast<uint32_t>(g * 256);
 #pragma unroll
     for (int kk = 0; kk < kKeys / 16; ++kk)
-      umma_f16_ts(p + 128, p + static_cast<uint32_t>(kk * 8),
-                  smem_desc_sw128(va + kk * 16 * 128, kHalfTile, 1024), idesc_o,
-                  (t > 1 || kk > 0) ? 1u : 0u);
-    umma_commit(&bars.v_empty[g]);
-    if (t + 2 >= nt) umma_commit(&bars.o_done[g]);
-    else if (!scores(t + 2)) return;
+      umma_f16_ts(p + 128, p + static_cast<uint32_t>(kk * 8), vd + ((kk * 16 * 128) >> 4), idesc,
+                  add || kk > 0 ? 1u : 0u);
+  }
+};
+
+// Two row tiles share every key tile: while the softmax works on one group's
+// S the tensor core runs the other's products.
+__device__ __forceinline__ void IssuePairs(const TileIssue& mma, const AttnBars& bars, int nt,
+                                           uint32_t* err) {
+  if (!mbar_wait(bars.q_full, 0, err) || !mbar_wait(&bars.k_full[0], 0, err)) return;
+  tc_fence_after_sync();
+#pragma unroll 1
+  for (int g = 0; g < 2; ++g) {
+    mma.Scores(g, g, 0);
+    umma_commit(&bars.s_full[g]);
+  }
+  umma_commit(&bars.k_empty[0]);
+#pragma unroll 1
+  for (int t = 0; t < nt; ++t) {
+    const int stage = t & 1, next = stage ^ 1;
+#pragma unroll 1
+    for (int g = 0; g < 2; ++g) {
+      if (!mbar_wait(&bars.p_full[g], static_cast<uint32_t>(t) & 1u, err) ||
+          (g == 0 && !mbar_wait(&bars.v_full[stage], static_cast<uint32_t>(t >> 1) & 1u, err)))
+        return;
+      tc_fence_after_sync();
+      mma.Values(g, stage, t > 0);
+      if (t + 1 == nt) {
+        umma_commit(&bars.o_done[g]);
+        continue;
+      }
+      if (g == 0 && !mbar_wait(&bars.k_full[next], static_cast<uint32_t>((t + 1) >> 1) & 1u, err)) return;
+      tc_fence_after_sync();
+      mma.Scores(g, g, next);
+      umma_commit(&bars.s_full[g]);
+    }
+    umma_commit(&bars.v_empty[stage]);
+    if (t + 1 < nt) umma_commit(&bars.k_empty[next]);
+  }
+}
+
+// One row tile: key tile t belongs to group t & 1.
+__device__ __forceinline__ void IssueSingle(const TileIssue& mma, const AttnBars& bars, int nt,
+                                            uint32_t* err) {
+  if (!mbar_wait(bars.q_full, 0, err)) return;
+  for (int t = -2; t < nt; ++t) {
+    const int g = t & 1;
+    if (t >= 0) {
+      const uint32_t phase = static_cast<uint32_t>(t >> 1) & 1u;
+      if (!mbar_wait(&bars.p_full[g], phase, err) || !mbar_wait(&bars.v_full[g], phase, err)) return;
+      tc_fence_after_sync();
+      mma.Values(g, g, t > 1);
+      umma_commit(&bars.v_empty[g]);
+    }
+    if (t + 2 < nt) {
+      if (!mbar_wait(&bars.k_full[g], static_cast<uint32_t>((t + 2) >> 1) & 1u, err)) return;
+      tc_fence_after_sync();
+      mma.Scores(g, 0, g);
+      umma_commit(&bars.s_full[g]);
+      umma_commit(&bars.k_empty[g]);
+    } else if (t >= 0) {
+      umma_commit(&bars.o_done[g]);
+    }
   }
 }
 
@@ -774,13 +862,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const int tile = args.tiles - 1 - static_cast<int>(blockIdx.x) / args.splits;
   const int split = static_cast<int>(blockIdx.x) % args.splits;
   const RowSpan span = SequenceRows(a.cu_rows, seq, a.rows, a.max_rows, a.err);
-  const int rows = span.count * a.group;  // at most 2^31 (host check)
+  const int rows = span.count * a.group.d;  // at most 2^31 (host check)
   const int row0 = tile * args.tile_rows;
   if (row0 >= rows) return;  // uniform over the CTA, before any barrier
   const int length = SequenceLength(a, seq);
   const bool pair = rows - row0 > kQ && args.tile_rows > kQ;
   const int here = min(rows - row0, args.tile_rows);
-  const int last_token = (row0 + here - 1) / a.group;
+  const int last_token = a.group(row0 + here - 1);
   const int reach = a.causal ? max(0, length - span.count + last_token + 1) : length;
   const int all_tiles = (reach + kKeys - 1) / kKeys;
   const int per = max(1, (all_tiles + args.splits - 1) / args.splits);
@@ -838,6 +926,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   float* part = parts > 1 ? args.parts + (item * args.splits + split) * TilePartFloats(args.tile_rows) : nullptr;
   const int stats_at = args.tile_rows * kCacheHeadDim;
 
+  if (warp >= kConvertWarp) registers_shrink<72>();
   if (warp == kLoadWarp) {
     // Lane i < 8 looks after slab i of a key tile; the first slab of a box
     // loads it.  Codes wait for the converters, one key tile ahead of them.
@@ -908,25 +997,34 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
   } else if (warp == kMmaWarp) {
     if (lane == 0 && nt > 0) {
-      if (pair) {
-        AttnArgs issue{};
-        issue.err = a.err;
-        (void)AttnIssue(issue, tmem, bars, AttnPhase{}, q_s, k_s, v_s, 2, nt);
-      } else {
-        IssueSingle(tmem, bars, q_s, k_s, v_s, nt, a.err);
-      }
+      const TileIssue mma(tmem, q_s, k_s, v_s);
+      if (pair) IssuePairs(mma, bars, nt, a.err);
+      else IssueSingle(mma, bars, nt, a.err);
     }
+    __syncwarp();
+    named_barrier(2, 256 + 32);  // O was read
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, 512);
   } else if (warp < kConvertWarp) {
-    // Query rows into the swizzled tiles, 16 lanes a row.
-    for (int r = tid >> 4; r < (pair ? 2 : 1) * kQ; r += 16) {
-      const int row = row0 + r, piece = tid & 15;
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (r < here)
-        x = *reinterpret_cast<const uint4*>(
-            a.q + static_cast<int64_t>(span.first + row / a.group) * a.ld_q +
-            (kv_head * a.group + row % a.group) * kCacheHeadDim + piece * 8);
-      *reinterpret_cast<uint4*>(q_s + (r >> 7) * kTile + (piece >> 3) * kHalfTile + (r & 127) * 128 +
-                                (((piece & 7) ^ (r & 7)) << 4)) = x;
+    registers_grow<184>();
+    // Query rows into the swizzled tiles, 16 lanes a row, all loads in flight.
+    const int piece = tid & 15;
+    uint4 rows_in[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int row = row0 + i * 16 + (tid >> 4), token = a.group(row);
+      rows_in[i] = make_uint4(0, 0, 0, 0);
+      if (row - row0 < here)
+        rows_in[i] = *reinterpret_cast<const uint4*>(
+            a.q + static_cast<int64_t>(span.first + token) * a.ld_q +
+            (kv_head * a.group.d + row - token * a.group.d) * kCacheHeadDim + piece * 8);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int r = i * 16 + (tid >> 4);
+      if (pair || i < 8)
+        *reinterpret_cast<uint4*>(q_s + (r >> 7) * kTile + (piece >> 3) * kHalfTile + (r & 127) * 128 +
+                                  (((piece & 7) ^ (r & 7)) << 4)) = rows_in[i];
     }
     fence_proxy_async_smem();
     mbar_arrive(&s.q_full);
@@ -938,9 +1036,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const uint32_t s_addr = tmem + static_cast<uint32_t>(g * 256) + lanes;
     const uint32_t o_addr = s_addr + 128;
     const int before = length - span.count;  // tokens that row token 0 has before it
-    const int seen = a.causal ? min(length, before + mine / a.group + 1) : length;
+    const int seen = a.causal ? min(length, before + a.group(mine) + 1) : length;
     // The fewest tokens that a row of this tile sees.
-    const int least = a.causal ? before + (mine - r) / a.group + 1 : length;
+    const int least = a.causal ? before + a.group(mine - r) + 1 : length;
     const int step = pair ? 1 : 2, first = pair ? 0 : g;
     float m = -INFINITY, l = 0.0f;
     int use = 0;
@@ -957,32 +1055,38 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
       for (int i = 0; i < kSlabs; ++i) bad |= slab[i].bad;
       const bool partial = token0 + kKeys > least || bad != 0;
-      const int valid = partial ? seen - token0 : kKeys;
+      uint32_t x[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_addr + c * 32, x[c]);
+      tmem_ld_wait();
+      if (partial) {
+        const int valid = seen - token0;
+#pragma unroll
+        for (int i = 0; i < kSlabs; ++i) {
+          const int slab_valid = slab[i].bad != 0 ? 0 : valid - i * 16;
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (j >= slab_valid) x[i >> 1][(i & 1) * 16 + j] = 0xFF800000u;
+        }
+      }
+      // A slab that the row sees nothing of must not bring a NaN scale.
+      auto scale_of = [&](int i) {
+        SlabScale k = slab[i];
+        if (partial && (k.bad != 0 || seen - token0 <= i * 16)) k.factor = 1.0f, k.shift = 0.0f;
+        return k;
+      };
       float top = -INFINITY;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t x[2][32];
-        tmem_ld_32x32b_x32(s_addr + c * 64, x[0]);
-        tmem_ld_32x32b_x32(s_addr + c * 64 + 32, x[1]);
-        tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t* v = &x[i >> 1][(i & 1) * 16];
-          const SlabScale k = slab[c * 4 + i];
-          if (partial) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (c * 64 + i * 16 + j >= valid || k.bad) v[j] = 0xFF800000u;
-          }
-          top = fmaxf(top, fmaf(Max16(v), k.factor, k.shift));
-        }
+      for (int i = 0; i < kSlabs; ++i) {
+        const SlabScale k = scale_of(i);
+        top = fmaxf(top, fmaf(Max16(&x[i >> 1][(i & 1) * 16]), k.factor, k.shift));
       }
       bool rescale = false;
       float alpha = 1.0f;
-      const bool grow = use == 0 ? top > m : top > m + kRescaleThreshold;
       if (use == 0) {
         m = top;
       } else {
+        const bool grow = top > m + kRescaleThreshold;
         rescale = __any_sync(0xFFFFFFFFu, grow);
         if (grow) {
           alpha = ex2_approx(m - top);
@@ -992,38 +1096,24 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const float base = m == -INFINITY ? 0.0f : m;
       float sum = 0.0f;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t x[2][32];
-        tmem_ld_32x32b_x32(s_addr + c * 64, x[0]);
-        tmem_ld_32x32b_x32(s_addr + c * 64 + 32, x[1]);
-        tmem_ld_wait();
+      for (int c = 0; c < 4; ++c) {
+        uint32_t packed[16];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t packed[16];
+        for (int i = 0; i < 2; ++i) {
+          const SlabScale k = scale_of(c * 2 + i);
+          const float shift = k.shift - base;
+          float p0 = 0.0f, p1 = 0.0f;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const SlabScale k = slab[c * 4 + h * 2 + i];
-            const float shift = k.shift - base;
-            float p0 = 0.0f, p1 = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 16; j += 2) {
-              float e0 = fmaf(__uint_as_float(x[h][i * 16 + j]), k.factor, shift);
-              float e1 = fmaf(__uint_as_float(x[h][i * 16 + j + 1]), k.factor, shift);
-              if (partial) {
-                const int key = c * 64 + h * 32 + i * 16 + j;
-                if (key >= valid || k.bad) e0 = -INFINITY;
-                if (key + 1 >= valid || k.bad) e1 = -INFINITY;
-              }
-              e0 = ex2_approx(e0);
-              e1 = ex2_approx(e1);
-              p0 += e0;
-              p1 += e1;
-              packed[i * 8 + j / 2] = pack_half2(e0, e1);
-            }
-            sum = fmaf(p0 + p1, k.inverse, sum);
+          for (int j = 0; j < 16; j += 2) {
+            const float e0 = ex2_approx(fmaf(__uint_as_float(x[c][i * 16 + j]), k.factor, shift));
+            const float e1 = ex2_approx(fmaf(__uint_as_float(x[c][i * 16 + j + 1]), k.factor, shift));
+            p0 += e0;
+            p1 += e1;
+            packed[i * 8 + j / 2] = pack_half2(e0, e1);
           }
-          tmem_st_32x32b_x16(s_addr + c * 32 + h * 16, packed);
+          sum = fmaf(p0 + p1, k.inverse, sum);
         }
+        tmem_st_32x32b_x16(s_addr + c * 16, packed);
       }
       if (rescale) {
         l *= alpha;
@@ -1044,124 +1134,150 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       mbar_arrive(&s.p_full[g]);
     }
 
-    // O of this warpgroup's tiles; in the single form the odd key tiles'
-    // half goes through shared memory (every MMA is done: the rings are idle).
-    const bool any = nt > first;
-    if (pair && any) ok = ok && mbar_wait(&s.o_done[g], 0, a.err);
+    // O of this warpgroup's tile.  In the single form the warpgroups have the
+    // even and the odd key tiles' parts of one tile: each takes half of the
+    // columns, the other's half comes through shared memory (every MMA is
+    // done by then, so the rings are idle).  Columns here: [col0, col0 + 32 n).
+    if (pair && nt > 0) ok = ok && mbar_wait(&s.o_done[g], 0, a.err);
     if (!pair && nt > 0) ok = ok && mbar_wait(&s.o_done[0], 0, a.err);
     if (!pair && nt > 1) ok = ok && mbar_wait(&s.o_done[1], 0, a.err);
     __syncwarp();
     tc_fence_after_sync();
-    constexpr int kPad = kCacheHeadDim + 4;
-    float* other = reinterpret_cast<float*>(k_s) + r * kPad;
+    const bool mine_any = nt > first, other_any = !pair && nt > 1 - first;
+    const int chunks = pair ? 4 : 2, col0 = pair ? 0 : g * 64;
+    float4* exchange = reinterpret_cast<float4*>(k_s);  // [group][16 vectors][128 rows]
+    float2* stats = reinterpret_cast<float2*>(v_s);     // [group][128 rows]
     float scale_mine = 1.0f, scale_other = 0.0f;
     if (!pair) {
-      float2* stats = reinterpret_cast<float2*>(k_s + kQ * kPad * sizeof(float)) + r;
-      if (g == 1) {
-        if (any) {
+      if (mine_any) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t x[32];
-            tmem_ld_32x32b_x32(o_addr + c * 32, x);
-            tmem_ld_wait();
-#pragma unroll
-            for (int j = 0; j < 32; j += 4)
-              *reinterpret_cast<uint4*>(other + c * 32 + j) = make_uint4(x[j], x[j + 1], x[j + 2], x[j + 3]);
-          }
-        }
-        *stats = make_float2(m, l);
-      }
-      named_barrier(1, 256);
-      if (g == 0) {
-        const float2 o = *stats;
-        const float top = fmaxf(m, o.x);
-        const float base = top == -INFINITY ? 0.0f : top;
-        scale_mine = ex2_approx(m - base);
-        scale_other = ex2_approx(o.x - base);
-        l = l * scale_mine + o.y * scale_other;
-        m = top;
-      }
-    }
-    if (pair || g == 0) {
-      const bool store = mine - row0 < here;
-      const float inv = part != nullptr ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-      const int at = mine - row0;  // row of this CTA
-      __half* dst = a.out + static_cast<int64_t>(span.first + mine / a.group) * a.ld_out +
-                    (kv_head * a.group + mine % a.group) * kCacheHeadDim;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t x[32];
-        float o[32];
-        if (nt > 0) {
-          tmem_ld_32x32b_x32(o_addr + c * 32, x);
+        for (int c = 0; c < 2; ++c) {
+          uint32_t x[32];
+          tmem_ld_32x32b_x32(o_addr + (64 - col0) + c * 32, x);
           tmem_ld_wait();
-        }
 #pragma unroll
-        for (int j = 0; j < 32; ++j) o[j] = nt > 0 ? __uint_as_float(x[j]) * scale_mine : 0.0f;
-        if (!pair && nt > 1) {
-#pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const float4 y = *reinterpret_cast<const float4*>(other + c * 32 + j);
-            o[j] = fmaf(y.x, scale_other, o[j]);
-            o[j + 1] = fmaf(y.y, scale_other, o[j + 1]);
-            o[j + 2] = fmaf(y.z, scale_other, o[j + 2]);
-            o[j + 3] = fmaf(y.w, scale_other, o[j + 3]);
-          }
-        }
-        if (!store) continue;
-        if (part != nullptr) {
-#pragma unroll
-          for (int j = 0; j < 32; j += 4)
-            *reinterpret_cast<float4*>(part + at * kCacheHeadDim + c * 32 + j) =
-                make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; j += 8)
-            *reinterpret_cast<uint4*>(dst + c * 32 + j) =
-                make_uint4(pack_half2(o[j] * inv, o[j + 1] * inv), pack_half2(o[j + 2] * inv, o[j + 3] * inv),
-                           pack_half2(o[j + 4] * inv, o[j + 5] * inv), pack_half2(o[j + 6] * inv, o[j + 7] * inv));
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<uint4*>(exchange + (g * 16 + c * 8 + j) * kQ + r) =
+                make_uint4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
         }
       }
-      if (part != nullptr && store) {
-        *reinterpret_cast<float2*>(part + stats_at + 2 * at) = make_float2(m, l);
-        __threadfence();
+      stats[g * kQ + r] = make_float2(m, l);
+      named_barrier(1, 256);
+      const float2 o = stats[(g ^ 1) * kQ + r];
+      const float top = fmaxf(m, o.x);
+      const float base = top == -INFINITY ? 0.0f : top;
+      scale_mine = ex2_approx(m - base);
+      scale_other = ex2_approx(o.x - base);
+      // In group order, so that both halves of a row divide by the same sum.
+      l = g == 0 ? fmaf(o.y, scale_other, l * scale_mine) : fmaf(l, scale_mine, o.y * scale_other);
+      m = top;
+    }
+    const int at = mine - row0;  // row of this CTA
+    if (part == nullptr) {
+      scale_mine = l == 0.0f ? 0.0f : scale_mine / l;
+      scale_other = l == 0.0f ? 0.0f : scale_other / l;
+    }
+    // Halves go through the query tile, idle too, so that rows leave whole.
+    uint8_t* stage = q_s + (pair ? g * kTile : 0);
+    for (int c = 0; c < chunks; ++c) {
+      const int col = col0 + c * 32;
+      uint32_t x[32];
+      float o[32];
+      if (mine_any) {
+        tmem_ld_32x32b_x32(o_addr + col, x);
+        tmem_ld_wait();
+      }
+#pragma unroll
+      for (int j = 0; j < 32; ++j) o[j] = mine_any ? __uint_as_float(x[j]) * scale_mine : 0.0f;
+      if (other_any) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float4 y = exchange[((g ^ 1) * 16 + c * 8 + j) * kQ + r];
+          o[4 * j] = fmaf(y.x, scale_other, o[4 * j]);
+          o[4 * j + 1] = fmaf(y.y, scale_other, o[4 * j + 1]);
+          o[4 * j + 2] = fmaf(y.z, scale_other, o[4 * j + 2]);
+          o[4 * j + 3] = fmaf(y.w, scale_other, o[4 * j + 3]);
+        }
+      }
+      if (part != nullptr) {  // vector v of all rows, then vector v + 1
+        if (at < here) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            reinterpret_cast<float4*>(part)[(col / 4 + j) * args.tile_rows + at] =
+                make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+        }
+      } else {
+        uint8_t* dst = stage + (col >> 6) * kHalfTile + r * 128;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int piece = ((col & 63) >> 3) + j;
+          *reinterpret_cast<uint4*>(dst + ((piece ^ (r & 7)) << 4)) =
+              make_uint4(pack_half2(o[8 * j], o[8 * j + 1]), pack_half2(o[8 * j + 2], o[8 * j + 3]),
+                         pack_half2(o[8 * j + 4], o[8 * j + 5]), pack_half2(o[8 * j + 6], o[8 * j + 7]));
+        }
       }
     }
-  }
-  tc_fence_before_sync();
-  __syncthreads();
-  if (warp == kMmaWarp) {
-    tc_fence_after_sync();
-    tmem_dealloc(tmem, 512);
-  }
-  if (part == nullptr) return;
-  // The last part to arrive joins all of them, in split order.
-  uint32_t* counter = args.counters + item;
-  if (tid == 0) {
-    __threadfence();
-    s.last = atomicAdd(counter, 1u) == static_cast<uint32_t>(parts - 1);
-    if (s.last) *counter = 0;
-  }
-  __syncthreads();
-  if (!s.last) return;
-  __threadfence();
-  const float* base_part = args.parts + item * args.splits * TilePartFloats(args.tile_rows);
-  for (int i = tid; i < here * (kCacheHeadDim / 4); i += kTileThreads) {
-    const int at = i / (kCacheHeadDim / 4), d = i % (kCacheHeadDim / 4) * 4;
-    float top = -INFINITY, sum = 0.0f;
-    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    tc_fence_before_sync();
+    named_barrier(2, 256 + 32);
+    auto out_row = [&](int r_) {
+      const int row = row0 + r_, token = a.group(row);
+      return a.out + static_cast<int64_t>(span.first + token) * a.ld_out +
+             (kv_head * a.group.d + row - token * a.group.d) * kCacheHeadDim;
+    };
+    if (part == nullptr) {
+      const int count = min(here, pair ? 2 * kQ : kQ);
 #pragma unroll 4
-    for (int x = 0; x < parts; ++x) {
-      const float* p = base_part + x * TilePartFloats(args.tile_rows);
-      const float2 ms = __ldcg(reinterpret_cast<const float2*>(p + stats_at + 2 * at));
-      const float4 y = __ldcg(reinterpret_cast<const float4*>(p + at * kCacheHeadDim + d));
-      JoinPart(&top, &sum, &v, ms, y);
+      for (int i = tid >> 4; i < count; i += 16)
+        *reinterpret_cast<uint4*>(out_row(i) + piece * 8) = *reinterpret_cast<const uint4*>(
+            q_s + (i >> 7) * kTile + (piece >> 3) * kHalfTile + (i & 127) * 128 + (((piece & 7) ^ (i & 7)) << 4));
+      return;
     }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const int row = row0 + at;
-    *reinterpret_cast<uint2*>(a.out + static_cast<int64_t>(span.first + row / a.group) * a.ld_out +
-                              (kv_head * a.group + row % a.group) * kCacheHeadDim + d) =
-        make_uint2(pack_half2(v.x * inv, v.y * inv), pack_half2(v.z * inv, v.w * inv));
+    if (at < here && (pair || g == 0))
+      *reinterpret_cast<float2*>(part + stats_at + 2 * at) = make_float2(m, l);
+    // The last part to arrive joins all of them, in split order.
+    __threadfence();
+    named_barrier(1, 256);
+    uint32_t* counter = args.counters + item;
+    if (tid == 0) {
+      __threadfence();
+      s.last = atomicAdd(counter, 1u) == static_cast<uint32_t>(parts - 1);
+      if (s.last) *counter = 0;
+    }
+    named_barrier(1, 256);
+    if (!s.last) return;
+    __threadfence();
+    const float* base_part = args.parts + item * args.splits * TilePartFloats(args.tile_rows);
+    for (int i = tid; i < 8 * args.tile_rows; i += 256) {
+      const int row = i & (args.tile_rows - 1), d16 = i / args.tile_rows;  // 16 columns of a row
+      if (row >= here) continue;
+      float top = -INFINITY, sum = 0.0f;
+      float o[16] = {};
+#pragma unroll 2
+      for (int x = 0; x < parts; ++x) {
+        const float* p = base_part + x * TilePartFloats(args.tile_rows);
+        const float2 ms = __ldcg(reinterpret_cast<const float2*>(p + stats_at + 2 * row));
+        float4 y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          y[j] = __ldcg(reinterpret_cast<const float4*>(p) + (d16 * 4 + j) * args.tile_rows + row);
+        const float2 f = JoinFactors(&top, &sum, ms);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          o[4 * j] = fmaf(y[j].x, f.y, o[4 * j] * f.x);
+          o[4 * j + 1] = fmaf(y[j].y, f.y, o[4 * j + 1] * f.x);
+          o[4 * j + 2] = fmaf(y[j].z, f.y, o[4 * j + 2] * f.x);
+          o[4 * j + 3] = fmaf(y[j].w, f.y, o[4 * j + 3] * f.x);
+        }
+      }
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      uint4* dst = reinterpret_cast<uint4*>(out_row(row) + d16 * 16);
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        dst[j] = make_uint4(pack_half2(o[8 * j] * inv, o[8 * j + 1] * inv),
+                            pack_half2(o[8 * j + 2] * inv, o[8 * j + 3] * inv),
+                            pack_half2(o[8 * j + 4] * inv, o[8 * j + 5] * inv),
+                            pack_half2(o[8 * j + 6] * inv, o[8 * j + 7] * inv));
+    }
   }
 }
 
@@ -1284,7 +1400,7 @@ int ov_attention_kv_cache(const ov_kv_cache* cache, const uint16_t* q, size_t ld
     RequireOnDevice(cu_rows, "cu_rows");
     RequireOnDevice(lengths, "lengths");
     if (workspace != nullptr) RequireOnDevice(workspace, "workspace");
-    CacheAttnArgs a;
+    CacheAttnArgs a{.group = FastDiv(static_cast<int>(heads / cache->kv_heads))};
     a.cache = c;
     a.q = reinterpret_cast<const __half*>(q);
     a.ld_q = static_cast<int64_t>(ld_q);
@@ -1296,7 +1412,6 @@ int ov_attention_kv_cache(const ov_kv_cache* cache, const uint16_t* q, size_t ld
     a.max_rows = static_cast<int>(std::min(max_rows, rows));
     a.max_length = static_cast<int>(max_length);
     a.heads = static_cast<int>(heads);
-    a.group = static_cast<int>(heads / cache->kv_heads);
     a.causal = causal != 0;
     a.scale_log2 = scale * 1.4426950408889634f;
     a.err = DeviceErrorWord();

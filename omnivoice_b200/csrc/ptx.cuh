@@ -512,6 +512,18 @@ __device__ __forceinline__ void named_barrier(uint32_t id, uint32_t threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
+// Moves this warpgroup's registers per thread to N (a multiple of 8); every
+// warp of the warpgroup calls it.  The sum over a block's warpgroups must not
+// exceed what the block was launched with.
+template <int N>
+__device__ __forceinline__ void registers_grow() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void registers_shrink() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 // Named barrier that also returns the OR of `v` over the `threads` threads
 // meeting at it.
 __device__ __forceinline__ bool named_barrier_or(uint32_t id, uint32_t threads, bool v) {
