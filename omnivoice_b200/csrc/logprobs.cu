@@ -241,33 +241,128 @@ __global__ void __launch_bounds__(kWarps * 32) logprobs_warp_kernel(const Logpro
 constexpr int kThreads = 512;
 constexpr int kKeys = 1024;      // room for passing values between prunings
 constexpr int kPruneAt = 512;
+constexpr int kVectors = 4;      // 16-byte vectors of a thread and chunk
 
-// Running maximum, Z and sum e^d d of what was read.
+// Running maximum, Z = sum 2^t and W = sum 2^t t of what was read, with
+// t = Row<T>::Exponent(x, m).
 struct RowStats {
   float m, z, w;
-  // To a maximum m2 >= m.
-  __device__ __forceinline__ void Rebase(float m2) {
-    if (m == -INFINITY) {
-      m = m2;
-      return;
-    }
-    const float d = m - m2, f = Exp2Approx(d * kLog2E);
-    w = f * fmaf(d, z, w);
-    z *= f;
-    m = m2;
+};
+
+// 16 bytes of logits, and how their exponent t = (x - m) log2(e) is formed.
+// For float32 the difference comes first: a mask of the type's lowest value
+// times log2(e) would overflow.  For halves it cannot, and one fused
+// multiply-add against Scaled(m) does.
+template <typename T>
+struct Row;
+
+template <>
+struct Row<float> {
+  static constexpr int kN = 4;
+  static __device__ __forceinline__ uint4 Closed() {  // all -inf
+    return make_uint4(0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u);
   }
-  __device__ __forceinline__ void Merge(RowStats o) {
-    const float top = MaxNan(m, o.m);
-    if (!(fabsf(top) < INFINITY)) {  // nothing yet, or no distribution
-      m = top;
-      return;
-    }
-    Rebase(top);
-    o.Rebase(top);
-    z += o.z;
-    w += o.w;
+  static __device__ __forceinline__ float Scaled(float m) { return m; }
+  static __device__ __forceinline__ float Exponent(float x, float scaled) {
+    return (x - scaled) * kLog2E;
+  }
+  // log p of a value, with log_z = log Z.
+  static __device__ __forceinline__ float LogProb(float x, float m, float log_z) {
+    return (x - m) - log_z;
+  }
+  static __device__ __forceinline__ float At(const uint4& q, int i) {
+    return __uint_as_float(i == 0 ? q.x : i == 1 ? q.y : i == 2 ? q.z : q.w);
+  }
+  // Exponent of the step from one maximum to another.
+  static __device__ __forceinline__ float Step(float from, float to) {
+    return (from - to) * kLog2E;
+  }
+  static __device__ __forceinline__ float Top(const uint4 (&q)[kVectors]) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kVectors; ++u)
+#pragma unroll
+      for (int i = 0; i < kN; ++i) top = MaxNan(top, At(q[u], i));
+    return top;
+  }
+  // Values of a vector above x, or at least x.
+  static __device__ __forceinline__ int Above(const uint4& q, float x, bool equal) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) n += equal ? At(q, i) >= x : At(q, i) > x;
+    return n;
   }
 };
+
+template <>
+struct Row<__half> {
+  static constexpr int kN = 8;
+  static __device__ __forceinline__ uint4 Closed() {
+    return make_uint4(0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u);
+  }
+  // Rounded by itself: a contracted product would make Step(m, m) its residue.
+  static __device__ __forceinline__ float Scaled(float m) { return __fmul_rn(m, kLog2E); }
+  static __device__ __forceinline__ float Exponent(float x, float scaled) {
+    return fmaf(x, kLog2E, -scaled);
+  }
+  static __device__ __forceinline__ float LogProb(float x, float m, float log_z) {
+    return fmaf(Exponent(x, Scaled(m)), 0.6931471805599453f, -log_z);
+  }
+  static __device__ __forceinline__ float At(const uint4& q, int i) {
+    const uint32_t w = i < 2 ? q.x : i < 4 ? q.y : i < 6 ? q.z : q.w;
+    return __half2float(__ushort_as_half(static_cast<uint16_t>(i & 1 ? w >> 16 : w)));
+  }
+  static __device__ __forceinline__ float Step(float from, float to) {
+    return Scaled(from) - Scaled(to);
+  }
+  static __device__ __forceinline__ __half2 Pair(uint32_t w) {
+    return *reinterpret_cast<const __half2*>(&w);
+  }
+  static __device__ __forceinline__ float Top(const uint4 (&q)[kVectors]) {
+    __half2 top = __half2half2(__ushort_as_half(0xFC00));
+#pragma unroll
+    for (int u = 0; u < kVectors; ++u) {
+      top = __hmax2_nan(top, __hmax2_nan(Pair(q[u].x), Pair(q[u].y)));
+      top = __hmax2_nan(top, __hmax2_nan(Pair(q[u].z), Pair(q[u].w)));
+    }
+    return MaxNan(__low2float(top), __high2float(top));
+  }
+  static __device__ __forceinline__ int Above(const uint4& q, float x, bool equal) {
+    const __half2 h = __float2half2_rn(x);  // a half to begin with
+    __half2 n;
+    if (equal)
+      n = __hadd2(__hadd2(__hge2(Pair(q.x), h), __hge2(Pair(q.y), h)),
+                  __hadd2(__hge2(Pair(q.z), h), __hge2(Pair(q.w), h)));
+    else
+      n = __hadd2(__hadd2(__hgt2(Pair(q.x), h), __hgt2(Pair(q.y), h)),
+                  __hadd2(__hgt2(Pair(q.z), h), __hgt2(Pair(q.w), h)));
+    return static_cast<int>(__low2float(n) + __high2float(n));
+  }
+};
+
+// To a maximum m >= s.m.
+template <typename T>
+__device__ __forceinline__ void Rebase(RowStats& s, float m) {
+  if (s.m != -INFINITY) {
+    const float d = fmaxf(Row<T>::Step(s.m, m), -16384.0f);
+    const float f = Exp2Approx(d);
+    s.w = f * fmaf(d, s.z, s.w);
+    s.z *= f;
+  }
+  s.m = m;
+}
+template <typename T>
+__device__ __forceinline__ void Merge(RowStats& s, RowStats o) {
+  const float top = MaxNan(s.m, o.m);
+  if (!(fabsf(top) < INFINITY)) {  // nothing yet, or no distribution
+    s.m = top;
+    return;
+  }
+  Rebase<T>(s, top);
+  Rebase<T>(o, top);
+  s.z += o.z;
+  s.w += o.w;
+}
 
 __device__ __forceinline__ uint32_t LoadCluster32(uint32_t address) {
   uint32_t v;
@@ -280,44 +375,16 @@ __device__ __forceinline__ uint64_t LoadCluster64(uint32_t address) {
   return v;
 }
 
-// 16 bytes of logits as floats.
-template <typename T>
-struct Vec;
-template <>
-struct Vec<float> {
-  static constexpr int kN = 4;
-  static __device__ __forceinline__ void Unpack(const uint4& q, float* x) {
-    x[0] = __uint_as_float(q.x);
-    x[1] = __uint_as_float(q.y);
-    x[2] = __uint_as_float(q.z);
-    x[3] = __uint_as_float(q.w);
-  }
-};
-template <>
-struct Vec<__half> {
-  static constexpr int kN = 8;
-  static __device__ __forceinline__ void Unpack(const uint4& q, float* x) {
-    const uint32_t r[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r[i]));
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
-    }
-  }
-};
-
 struct LongShared {
   uint64_t keys[kKeys];
   uint64_t sorted[8 * kMaxTopK];
   uint64_t warp_key[kThreads / 32];
-  float kth[kThreads / 32];
+  float fourth[kThreads / 32];
   RowStats stats[kThreads / 32];
   int ahead[kThreads / 32];
   RowStats total;
   int total_ahead;
   int count;
-  int found;
   float threshold;
 };
 
@@ -328,6 +395,7 @@ __device__ __forceinline__ void Prune(LongShared& s, int k) {
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const uint64_t key = s.keys[i];
     int r = 0;
+#pragma unroll 4
     for (int j = 0; j < n; ++j) r += s.keys[j] > key ? 1 : 0;
     if (r < k) s.sorted[r] = key;
   }
@@ -340,11 +408,11 @@ __device__ __forceinline__ void Prune(LongShared& s, int k) {
   __syncthreads();
 }
 
-template <typename T, int kU>
+template <typename T>
 __global__ void __launch_bounds__(kThreads, 2)
     logprobs_long_kernel(const LogprobArgs a, int cluster) {
-  constexpr int kE = Vec<T>::kN;
-  constexpr int kN = kU * kE;
+  using R = Row<T>;
+  constexpr int kE = R::kN;
   __shared__ LongShared s;
   pdl_trigger();
   pdl_wait();
@@ -356,79 +424,107 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int64_t out = codebook * a.rows + row;
   const T* src = static_cast<const T*>(a.logits) + row * a.ld + static_cast<int64_t>(codebook) * a.vocab;
   const int k = a.top_k;
+  // Up to the first 16-byte boundary and behind the last whole vector: the
+  // row's ends, read value by value, the first end before and the last one
+  // behind the vectors (alternatives arrive by ascending index).
+  const int head = min(a.vocab, static_cast<int>((16u - (reinterpret_cast<uintptr_t>(src) & 15u)) % 16u /
+                                                 sizeof(T)));
+  const uint4* base = reinterpret_cast<const uint4*>(src + head);
+  const int vectors = (a.vocab - head) / kE;
+  const int per = (vectors + cluster - 1) / cluster;
+  const int begin = part * per, end = min(vectors, begin + per);
+  auto load = [&](int v0, uint4 (&q)[kVectors]) {
+#pragma unroll
+    for (int u = 0; u < kVectors; ++u) {
+      const int v = v0 + u * kThreads + tid;
+      q[u] = v < end ? __ldg(base + v) : R::Closed();
+    }
+  };
+  uint4 next[kVectors];
+  load(begin, next);
   const int target = Target(a, out, tid == 0 && part == 0);
-  const float xt = target >= 0 ? ToFloat(src[target]) : INFINITY;
+  const float xt = target >= 0 ? ToFloat(src[target]) : 0.0f;
+  const bool ranks = a.rank != nullptr && target >= 0;
   if (tid == 0) {
     s.count = 0;
     s.threshold = -INFINITY;
   }
-  // Vectors of 16 aligned bytes; vector v holds values [kE v - skip, ...).
-  const int skip = static_cast<int>((reinterpret_cast<uintptr_t>(src) & 15u) / sizeof(T));
-  const uint4* base = reinterpret_cast<const uint4*>(src - skip);
-  const int vectors = (skip + a.vocab + kE - 1) / kE;
-  const int per = (vectors + cluster - 1) / cluster;
-  const int begin = part * per, end = min(vectors, begin + per);
-
-  auto load = [&](int v, float* x) {
-    const int j = v * kE - skip;
-    if (v < end && j >= 0 && j + kE <= a.vocab) {
-      Vec<T>::Unpack(base[v], x);
-    } else {
-#pragma unroll
-      for (int e = 0; e < kE; ++e)
-        x[e] = v < end && j + e >= 0 && j + e < a.vocab ? ToFloat(src[j + e]) : -INFINITY;
-    }
-  };
+  __syncthreads();
 
   RowStats st = {-INFINITY, 0.0f, 0.0f};
   int ahead = 0;
-  bool first = true;
-  for (int v0 = begin; v0 < end; v0 += kThreads * kU) {
-    float x[kN];
-#pragma unroll
-    for (int u = 0; u < kU; ++u) load(v0 + u * kThreads + tid, x + u * kE);
-    float top = x[0];
-#pragma unroll
-    for (int i = 1; i < kN; ++i) top = MaxNan(top, x[i]);
+  auto grow = [&](float top) {  // NaN or +inf stays: no distribution
     const float grown = MaxNan(st.m, top);
-    if (grown != st.m) {
-      if (fabsf(grown) < INFINITY) st.Rebase(grown);
-      else st.m = grown;  // NaN or +inf: no distribution
-    }
+    if (grown == st.m) return;
+    if (fabsf(grown) < INFINITY) Rebase<T>(st, grown);
+    else st.m = grown;
+  };
+  // One value of the row's ends, for threads below 8.
+  auto scalar = [&](int j, float threshold) {
+    const float x = ToFloat(src[j]);
+    grow(x);
     if (fabsf(st.m) < INFINITY) {
+      const float t = fmaxf(R::Exponent(x, R::Scaled(st.m)), -16384.0f);
+      const float p = Exp2Approx(t);
+      st.z += p;
+      st.w = fmaf(p, t, st.w);
+    }
+    ahead += ranks && (x > xt || (x == xt && j < target)) ? 1 : 0;
+    if (k > 0 && x > threshold) s.keys[atomicAdd(&s.count, 1)] = AlternativeKey(x, j);
+  };
+  if (part == 0 && tid < head) scalar(tid, -INFINITY);
+  bool first = true;
+  for (int v0 = begin; v0 < end; v0 += kThreads * kVectors) {
+    uint4 q[kVectors];
 #pragma unroll
-      for (int i = 0; i < kN; ++i) {
-        const float d = fmaxf(x[i] - st.m, -1e30f);
-        const float e = Exp2Approx(d * kLog2E);
-        st.z += e;
-        st.w = fmaf(e, d, st.w);
+    for (int u = 0; u < kVectors; ++u) q[u] = next[u];
+    if (v0 + kThreads * kVectors < end) load(v0 + kThreads * kVectors, next);
+    const float top = R::Top(q);
+    grow(top);
+    if (fabsf(st.m) < INFINITY) {
+      const float scaled = R::Scaled(st.m);
+#pragma unroll
+      for (int u = 0; u < kVectors; ++u) {
+        float z = 0.0f, w = 0.0f;  // of one vector: longer sums lose less
+#pragma unroll
+        for (int e = 0; e < kE; ++e) {
+          // Finite, so that a closed token's 0 * t is 0.
+          const float t = fmaxf(R::Exponent(R::At(q[u], e), scaled), -16384.0f);
+          const float p = Exp2Approx(t);
+          z += p;
+          w = fmaf(p, t, w);
+        }
+        st.z += z;
+        st.w += w;
       }
     }
-    if (a.rank != nullptr) {
+    if (ranks) {
 #pragma unroll
-      for (int u = 0; u < kU; ++u) {
-        const int v = v0 + u * kThreads + tid;
-        const int j = v * kE - skip;
+      for (int u = 0; u < kVectors; ++u) {
+        const int v = v0 + u * kThreads + tid, j = head + v * kE;
+        if (v >= end) continue;
+        const bool before = j + kE <= target;
+        if (before || j > target) {
+          ahead += R::Above(q[u], xt, before);
+        } else {  // the target's vector
 #pragma unroll
-        for (int e = 0; e < kE; ++e) ahead += x[u * kE + e] > xt ? 1 : 0;
-        if (v < end && j < target) {  // equal values ahead of the target
-#pragma unroll
-          for (int e = 0; e < kE; ++e)
-            ahead += x[u * kE + e] == xt && j + e < target && j + e >= 0 ? 1 : 0;
+          for (int e = 0; e < kE; ++e) {
+            const float x = R::At(q[u], e);
+            ahead += x > xt || (x == xt && j + e < target) ? 1 : 0;
+          }
         }
       }
     }
     if (k == 0) continue;
-    // The first values take their threshold from the threads' maxima: k
-    // lanes of a warp hold a value of at least its k-th greatest maximum.
+    // The first values take their threshold from the threads' maxima: in each
+    // of ceil(k / 4) warps four lanes hold a value of at least the warp's
+    // fourth greatest maximum.
     float threshold;
     if (first) {
-      const float kth = WarpKth(top, k);
-      if (lane == 0) s.kth[warp] = kth;
+      const float fourth = WarpKth(top, 4);
+      if (lane == 0) s.fourth[warp] = fourth;
       __syncthreads();
-      threshold = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < kThreads / 32; ++i) threshold = fmaxf(threshold, s.kth[i]);
+      threshold = WarpKth(lane < kThreads / 32 ? s.fourth[lane] : -INFINITY, (k + 3) / 4);
     } else {
       threshold = s.threshold;
     }
@@ -436,14 +532,14 @@ __global__ void __launch_bounds__(kThreads, 2)
     bool crowded = first;
     if (top > threshold || (first && top == threshold)) {
 #pragma unroll
-      for (int u = 0; u < kU; ++u) {
-        const int j = (v0 + u * kThreads + tid) * kE - skip;
+      for (int u = 0; u < kVectors; ++u) {
+        const int j = head + (v0 + u * kThreads + tid) * kE;
 #pragma unroll
         for (int e = 0; e < kE; ++e) {
-          const float v = x[u * kE + e];
-          if (v > threshold || (first && v == threshold && v > -INFINITY)) {
+          const float x = R::At(q[u], e);
+          if (x > threshold || (first && x == threshold && x > -INFINITY)) {
             const int at = atomicAdd(&s.count, 1);
-            if (at < kKeys) s.keys[at] = AlternativeKey(v, j + e);
+            if (at < kKeys) s.keys[at] = AlternativeKey(x, j + e);
             crowded |= at >= kPruneAt;
           }
         }
@@ -453,18 +549,18 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (s.count > kKeys) {
         // No room (many equal values, or rising ones): the k greatest of
         // these and of the keys from before, one after the other.
-        const int chunk = v0 * kE - skip;  // first index of these values
+        const int low = head + v0 * kE;  // these values' indices
+        const int high = head + min(end, v0 + kThreads * kVectors) * kE;
         uint64_t last = ~uint64_t{0};
         for (int r = 0; r < k; ++r) {
           uint64_t best = 0;
           for (int i = tid; i < kKeys; i += kThreads) {
             const uint64_t key = s.keys[i];
-            if (KeyIndex(key) < chunk && key < last && key > best) best = key;
+            if (KeyIndex(key) < low && key < last && key > best) best = key;
           }
-#pragma unroll
-          for (int i = 0; i < kN; ++i) {
-            const int j = (v0 + (i / kE) * kThreads + tid) * kE - skip + i % kE;
-            const uint64_t key = x[i] > -INFINITY ? AlternativeKey(x[i], j) : 0;
+          for (int j = low + tid; j < high; j += kThreads) {
+            const float x = ToFloat(src[j]);
+            const uint64_t key = x > -INFINITY ? AlternativeKey(x, j) : 0;
             if (key < last && key > best) best = key;
           }
           best = WarpMaxKey(best);
@@ -488,6 +584,10 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     first = false;
   }
+  if (part == cluster - 1) {
+    const int at = head + vectors * kE + tid;
+    if (at < a.vocab) scalar(at, s.threshold);
+  }
 
   // The CTA's sums, in a fixed order.
 #pragma unroll
@@ -496,7 +596,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     other.m = __shfl_xor_sync(0xFFFFFFFFu, st.m, o);
     other.z = __shfl_xor_sync(0xFFFFFFFFu, st.z, o);
     other.w = __shfl_xor_sync(0xFFFFFFFFu, st.w, o);
-    st.Merge(other);
+    Merge<T>(st, other);
   }
   ahead = __reduce_add_sync(0xFFFFFFFFu, ahead);
   if (lane == 0) {
@@ -505,15 +605,26 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   __syncthreads();
   if (k > 0) Prune(s, k);
-  if (tid == 0) {
-    RowStats total = s.stats[0];
-    int sum = s.ahead[0];
-    for (int i = 1; i < kThreads / 32; ++i) {
-      total.Merge(s.stats[i]);
-      sum += s.ahead[i];
+  if (warp == 0) {
+    RowStats total = {-INFINITY, 0.0f, 0.0f};
+    int sum = 0;
+    if (lane < kThreads / 32) {
+      total = s.stats[lane];
+      sum = s.ahead[lane];
     }
-    s.total = total;
-    s.total_ahead = sum;
+#pragma unroll
+    for (int o = kThreads / 64; o > 0; o >>= 1) {
+      RowStats other;
+      other.m = __shfl_xor_sync(0xFFFFFFFFu, total.m, o);
+      other.z = __shfl_xor_sync(0xFFFFFFFFu, total.z, o);
+      other.w = __shfl_xor_sync(0xFFFFFFFFu, total.w, o);
+      Merge<T>(total, other);
+    }
+    sum = __reduce_add_sync(0xFFFFFFFFu, sum);
+    if (lane == 0) {
+      s.total = total;
+      s.total_ahead = sum;
+    }
   }
   if (cluster > 1) {
     __syncthreads();
@@ -544,7 +655,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           o.m = __uint_as_float(LoadCluster32(at));
           o.z = __uint_as_float(LoadCluster32(at + 4));
           o.w = __uint_as_float(LoadCluster32(at + 8));
-          total.Merge(o);
+          Merge<T>(total, o);
           sum += static_cast<int>(LoadCluster32(mapa_shared(smem_u32(&s.total_ahead), peer)));
         }
         s.total = total;
@@ -563,14 +674,15 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   const float log_z = logf(total.z);
   if (tid == 0) {
-    a.logprob[out] = target >= 0 ? (xt - total.m) - log_z : 0.0f;
-    if (a.entropy != nullptr) a.entropy[out] = log_z - total.w / total.z;
+    a.logprob[out] = target >= 0 ? R::LogProb(xt, total.m, log_z) : 0.0f;
+    if (a.entropy != nullptr)
+      a.entropy[out] = fmaf(total.w / total.z, -0.6931471805599453f, log_z);
     if (a.rank != nullptr) a.rank[out] = target >= 0 ? s.total_ahead : -1;
   }
   const int n = min(s.count, k);
   if (tid < n) {
     a.top_ids[out * k + tid] = KeyIndex(s.keys[tid]);
-    a.top_logprobs[out * k + tid] = (KeyValue(s.keys[tid]) - total.m) - log_z;
+    a.top_logprobs[out * k + tid] = R::LogProb(KeyValue(s.keys[tid]), total.m, log_z);
   }
   // Fewer than top_k open tokens: closed ones by index.
   if (warp == 0 && n < k) {
@@ -603,9 +715,9 @@ void LaunchLogprobs(const LogprobArgs& a, cudaStream_t stream) {
   // vectors for all of its threads.
   unsigned cluster = 1;
   while (cluster < 8 && items * cluster * 2 <= 2 * SmCount() &&
-         a.vocab >= static_cast<int>(cluster) * 2 * kThreads * Vec<T>::kN)
+         a.vocab >= static_cast<int>(cluster) * 2 * kThreads * Row<T>::kN)
     cluster *= 2;
-  LaunchEx(logprobs_long_kernel<T, 16 / Vec<T>::kN>, dim3(static_cast<unsigned>(items) * cluster),
+  LaunchEx(logprobs_long_kernel<T>, dim3(static_cast<unsigned>(items) * cluster),
            dim3(kThreads), 0, stream, what, cluster, a, static_cast<int>(cluster));
 }
 
