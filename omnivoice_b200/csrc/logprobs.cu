@@ -240,8 +240,7 @@ __global__ void __launch_bounds__(kWarps * 32) logprobs_warp_kernel(const Logpro
 
 constexpr int kThreads = 512;
 constexpr int kKeys = 1024;      // room for passing values between prunings
-constexpr int kPruneAt = 512;
-constexpr int kVectors = 4;      // 16-byte vectors of a thread and chunk
+constexpr int kVectors = 4;      // 16-byte vectors of a thread and chunk (Row::Top takes four)
 
 // Running maximum, Z = sum 2^t and W = sum 2^t t of what was read, with
 // t = Row<T>::Exponent(x, m).
@@ -277,13 +276,11 @@ struct Row<float> {
   static __device__ __forceinline__ float Step(float from, float to) {
     return (from - to) * kLog2E;
   }
+  static __device__ __forceinline__ float Top(const uint4& q) {
+    return MaxNan(MaxNan(At(q, 0), At(q, 1)), MaxNan(At(q, 2), At(q, 3)));
+  }
   static __device__ __forceinline__ float Top(const uint4 (&q)[kVectors]) {
-    float top = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < kVectors; ++u)
-#pragma unroll
-      for (int i = 0; i < kN; ++i) top = MaxNan(top, At(q[u], i));
-    return top;
+    return MaxNan(MaxNan(Top(q[0]), Top(q[1])), MaxNan(Top(q[2]), Top(q[3])));
   }
   // Values of a vector above x, or at least x.
   static __device__ __forceinline__ int Above(const uint4& q, float x, bool equal) {
@@ -318,13 +315,16 @@ struct Row<__half> {
   static __device__ __forceinline__ __half2 Pair(uint32_t w) {
     return *reinterpret_cast<const __half2*>(&w);
   }
+  static __device__ __forceinline__ __half2 Top2(const uint4& q) {
+    return __hmax2_nan(__hmax2_nan(Pair(q.x), Pair(q.y)), __hmax2_nan(Pair(q.z), Pair(q.w)));
+  }
+  static __device__ __forceinline__ float Top(const uint4& q) {
+    const __half2 top = Top2(q);
+    return MaxNan(__low2float(top), __high2float(top));
+  }
   static __device__ __forceinline__ float Top(const uint4 (&q)[kVectors]) {
-    __half2 top = __half2half2(__ushort_as_half(0xFC00));
-#pragma unroll
-    for (int u = 0; u < kVectors; ++u) {
-      top = __hmax2_nan(top, __hmax2_nan(Pair(q[u].x), Pair(q[u].y)));
-      top = __hmax2_nan(top, __hmax2_nan(Pair(q[u].z), Pair(q[u].w)));
-    }
+    const __half2 top = __hmax2_nan(__hmax2_nan(Top2(q[0]), Top2(q[1])),
+                                    __hmax2_nan(Top2(q[2]), Top2(q[3])));
     return MaxNan(__low2float(top), __high2float(top));
   }
   static __device__ __forceinline__ int Above(const uint4& q, float x, bool equal) {
@@ -459,6 +459,10 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (fabsf(grown) < INFINITY) Rebase<T>(st, grown);
     else st.m = grown;
   };
+  auto push = [&](float x, int j) {
+    const int at = atomicAdd(&s.count, 1);
+    if (at < kKeys) s.keys[at] = AlternativeKey(x, j);
+  };
   // One value of the row's ends, for threads below 8.
   auto scalar = [&](int j, float threshold) {
     const float x = ToFloat(src[j]);
@@ -470,11 +474,53 @@ __global__ void __launch_bounds__(kThreads, 2)
       st.w = fmaf(p, t, st.w);
     }
     ahead += ranks && (x > xt || (x == xt && j < target)) ? 1 : 0;
-    if (k > 0 && x > threshold) s.keys[atomicAdd(&s.count, 1)] = AlternativeKey(x, j);
+    if (k > 0 && x > threshold) push(x, j);
   };
-  if (part == 0 && tid < head) scalar(tid, -INFINITY);
-  bool first = true;
-  for (int v0 = begin; v0 < end; v0 += kThreads * kVectors) {
+  // Leaves the k best so far in order in s.keys, and their threshold.  Values
+  // [low, high) came since the last time.
+  auto settle = [&](int low, int high) {
+    __syncthreads();
+    if (s.count > kKeys) {
+      // No room (many equal values, or rising ones): the best of these and of
+      // the keys from before, one after the other.
+      uint64_t last = ~uint64_t{0};
+      for (int r = 0; r < k; ++r) {
+        uint64_t best = 0;
+        for (int i = tid; i < kKeys; i += kThreads) {
+          const uint64_t key = s.keys[i];
+          if (KeyIndex(key) < low && key < last && key > best) best = key;
+        }
+        for (int j = low + tid; j < high; j += kThreads) {
+          const float x = ToFloat(src[j]);
+          const uint64_t key = x > -INFINITY ? AlternativeKey(x, j) : 0;
+          if (key < last && key > best) best = key;
+        }
+        best = WarpMaxKey(best);
+        if (lane == 0) s.warp_key[warp] = best;
+        __syncthreads();
+        last = 0;
+#pragma unroll
+        for (int i = 0; i < kThreads / 32; ++i) last = max(last, s.warp_key[i]);
+        if (tid == 0) s.sorted[r] = last;  // never 0: more than kKeys values passed
+        __syncthreads();
+      }
+      if (tid < k) s.keys[tid] = s.sorted[tid];
+      if (tid == 0) {
+        s.count = k;
+        s.threshold = KeyValue(s.sorted[k - 1]);
+      }
+      __syncthreads();
+    } else {
+      Prune(s, k);
+    }
+  };
+  if (part == 0) {
+    if (tid < head) scalar(tid, -INFINITY);
+    __syncthreads();  // the row's first keys are stored, whatever follows
+  }
+  int settled = head + begin * kE;  // values below are in order in s.keys
+  int chunk = 0;
+  for (int v0 = begin; v0 < end; v0 += kThreads * kVectors, ++chunk) {
     uint4 q[kVectors];
 #pragma unroll
     for (int u = 0; u < kVectors; ++u) q[u] = next[u];
@@ -520,6 +566,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     // of ceil(k / 4) warps four lanes hold a value of at least the warp's
     // fourth greatest maximum.
     float threshold;
+    const bool first = chunk == 0;
     if (first) {
       const float fourth = WarpKth(top, 4);
       if (lane == 0) s.fourth[warp] = fourth;
@@ -529,65 +576,31 @@ __global__ void __launch_bounds__(kThreads, 2)
       threshold = s.threshold;
     }
     // Later values lose to an equal earlier one, so they have to be greater.
-    bool crowded = first;
-    if (top > threshold || (first && top == threshold)) {
+    auto passes = [&](float x) {
+      return x > threshold || (first && x == threshold && x > -INFINITY);
+    };
+    if (passes(top)) {
 #pragma unroll
       for (int u = 0; u < kVectors; ++u) {
+        if (!passes(R::Top(q[u]))) continue;
         const int j = head + (v0 + u * kThreads + tid) * kE;
 #pragma unroll
         for (int e = 0; e < kE; ++e) {
           const float x = R::At(q[u], e);
-          if (x > threshold || (first && x == threshold && x > -INFINITY)) {
-            const int at = atomicAdd(&s.count, 1);
-            if (at < kKeys) s.keys[at] = AlternativeKey(x, j + e);
-            crowded |= at >= kPruneAt;
-          }
+          if (passes(x)) push(x, j + e);
         }
       }
     }
-    if (__syncthreads_or(crowded)) {
-      if (s.count > kKeys) {
-        // No room (many equal values, or rising ones): the k greatest of
-        // these and of the keys from before, one after the other.
-        const int low = head + v0 * kE;  // these values' indices
-        const int high = head + min(end, v0 + kThreads * kVectors) * kE;
-        uint64_t last = ~uint64_t{0};
-        for (int r = 0; r < k; ++r) {
-          uint64_t best = 0;
-          for (int i = tid; i < kKeys; i += kThreads) {
-            const uint64_t key = s.keys[i];
-            if (KeyIndex(key) < low && key < last && key > best) best = key;
-          }
-          for (int j = low + tid; j < high; j += kThreads) {
-            const float x = ToFloat(src[j]);
-            const uint64_t key = x > -INFINITY ? AlternativeKey(x, j) : 0;
-            if (key < last && key > best) best = key;
-          }
-          best = WarpMaxKey(best);
-          if (lane == 0) s.warp_key[warp] = best;
-          __syncthreads();
-          last = 0;
-#pragma unroll
-          for (int i = 0; i < kThreads / 32; ++i) last = max(last, s.warp_key[i]);
-          if (tid == 0) s.sorted[r] = last;  // never 0: more than kKeys values passed
-          __syncthreads();
-        }
-        if (tid < k) s.keys[tid] = s.sorted[tid];
-        if (tid == 0) {
-          s.count = k;
-          s.threshold = KeyValue(s.sorted[k - 1]);
-        }
-        __syncthreads();
-      } else {
-        Prune(s, k);
-      }
+    // After chunks 1, 2, 4, 8, ...: about top_k values pass in between.
+    if ((chunk & (chunk + 1)) == 0) {
+      const int high = head + min(end, v0 + kThreads * kVectors) * kE;
+      settle(settled, high);
+      settled = high;
     }
-    first = false;
   }
-  if (part == cluster - 1) {
-    const int at = head + vectors * kE + tid;
-    if (at < a.vocab) scalar(at, s.threshold);
-  }
+  const bool row_end = part == cluster - 1;
+  if (row_end && head + vectors * kE + tid < a.vocab) scalar(head + vectors * kE + tid, s.threshold);
+  if (k > 0) settle(settled, row_end ? a.vocab : head + end * kE);
 
   // The CTA's sums, in a fixed order.
 #pragma unroll
@@ -604,7 +617,6 @@ __global__ void __launch_bounds__(kThreads, 2)
     s.ahead[warp] = ahead;
   }
   __syncthreads();
-  if (k > 0) Prune(s, k);
   if (warp == 0) {
     RowStats total = {-INFINITY, 0.0f, 0.0f};
     int sum = 0;
