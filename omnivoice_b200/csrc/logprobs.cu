@@ -99,6 +99,19 @@ __device__ __forceinline__ float WarpKth(float v, int k) {
   return __shfl_sync(0xFFFFFFFFu, v, k - 1);
 }
 
+// The same for a small k, one maximum after the other.
+__device__ __forceinline__ float WarpKthOfFew(float v, int k) {
+  const uint32_t u = __float_as_uint(v);
+  uint32_t key = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  uint32_t top = __reduce_max_sync(0xFFFFFFFFu, key);
+  for (int i = 1; i < k; ++i) {
+    const uint32_t holders = __ballot_sync(0xFFFFFFFFu, key == top);
+    if ((threadIdx.x & 31) == __ffs(holders) - 1) key = 0;
+    top = __reduce_max_sync(0xFFFFFFFFu, key);
+  }
+  return __uint_as_float((top & 0x80000000u) ? (top & 0x7FFFFFFFu) : ~top);
+}
+
 // What a row without a distribution gives.
 __device__ __forceinline__ void StoreNothing(const LogprobArgs& a, int64_t out, int lane) {
   const float nan = __uint_as_float(0x7FC00000u);
@@ -238,7 +251,7 @@ __global__ void __launch_bounds__(kWarps * 32) logprobs_warp_kernel(const Logpro
 
 // ------------------------------ long rows: one CTA, or a cluster, per item
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
 constexpr int kKeys = 1024;      // room for passing values between prunings
 constexpr int kVectors = 4;      // 16-byte vectors of a thread and chunk (Row::Top takes four)
 
@@ -282,12 +295,27 @@ struct Row<float> {
   static __device__ __forceinline__ float Top(const uint4 (&q)[kVectors]) {
     return MaxNan(MaxNan(Top(q[0]), Top(q[1])), MaxNan(Top(q[2]), Top(q[3])));
   }
-  // Values of a vector above x, or at least x.
-  static __device__ __forceinline__ int Above(const uint4& q, float x, bool equal) {
+  // Values above x (kEqual: or equal to it).
+  template <bool kEqual>
+  static __device__ __forceinline__ int Above(const uint4 (&q)[kVectors], float x) {
     int n = 0;
 #pragma unroll
-    for (int i = 0; i < kN; ++i) n += equal ? At(q, i) >= x : At(q, i) > x;
+    for (int u = 0; u < kVectors; ++u)
+#pragma unroll
+      for (int i = 0; i < kN; ++i) n += kEqual ? At(q[u], i) >= x : At(q[u], i) > x;
     return n;
+  }
+  // Bit i: value i is above x.
+  static __device__ __forceinline__ uint32_t MaskAbove(const uint4& q, float x) {
+    uint32_t mask = 0;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) mask |= At(q, i) > x ? 1u << i : 0u;
+    return mask;
+  }
+  // The greatest value below x.
+  static __device__ __forceinline__ float Below(float x) {
+    return __uint_as_float(x > 0.0f ? __float_as_uint(x) - 1
+                                    : x == 0.0f ? 0x80000001u : __float_as_uint(x) + 1);
   }
 };
 
@@ -327,16 +355,26 @@ struct Row<__half> {
                                     __hmax2_nan(Top2(q[2]), Top2(q[3])));
     return MaxNan(__low2float(top), __high2float(top));
   }
-  static __device__ __forceinline__ int Above(const uint4& q, float x, bool equal) {
+  template <bool kEqual>
+  static __device__ __forceinline__ int Above(const uint4 (&q)[kVectors], float x) {
     const __half2 h = __float2half2_rn(x);  // a half to begin with
-    __half2 n;
-    if (equal)
-      n = __hadd2(__hadd2(__hge2(Pair(q.x), h), __hge2(Pair(q.y), h)),
-                  __hadd2(__hge2(Pair(q.z), h), __hge2(Pair(q.w), h)));
-    else
-      n = __hadd2(__hadd2(__hgt2(Pair(q.x), h), __hgt2(Pair(q.y), h)),
-                  __hadd2(__hgt2(Pair(q.z), h), __hgt2(Pair(q.w), h)));
+    auto test = [&](uint32_t w) { return kEqual ? __hge2(Pair(w), h) : __hgt2(Pair(w), h); };
+    __half2 n = __half2half2(__ushort_as_half(0));
+#pragma unroll
+    for (int u = 0; u < kVectors; ++u)
+      n = __hadd2(n, __hadd2(__hadd2(test(q[u].x), test(q[u].y)), __hadd2(test(q[u].z), test(q[u].w))));
     return static_cast<int>(__low2float(n) + __high2float(n));
+  }
+  static __device__ __forceinline__ uint32_t MaskAbove(const uint4& q, float x) {
+    const __half2 h = __float2half2_rn(x);
+    const uint32_t m = (__hgt2_mask(Pair(q.x), h) & 0x00020001u) | (__hgt2_mask(Pair(q.y), h) & 0x00080004u) |
+                       (__hgt2_mask(Pair(q.z), h) & 0x00200010u) | (__hgt2_mask(Pair(q.w), h) & 0x00800040u);
+    return (m | (m >> 16)) & 0xFFu;
+  }
+  static __device__ __forceinline__ float Below(float x) {
+    const uint16_t h = __half_as_ushort(__float2half_rn(x));
+    return __half2float(__ushort_as_half(static_cast<uint16_t>(
+        x > 0.0f ? h - 1 : x == 0.0f ? 0x8001 : h + 1)));
   }
 };
 
@@ -391,13 +429,17 @@ struct LongShared {
 // Leaves the top_k greatest of the `count` keys in order in keys[0 ..) and
 // sets count and threshold.  Every thread calls it, after a barrier.
 __device__ __forceinline__ void Prune(LongShared& s, int k) {
-  const int n = s.count;
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const uint64_t key = s.keys[i];
+  // Four lanes count the keys ahead of one.
+  const int n = s.count, lanes = threadIdx.x & 3;
+  for (int i0 = 0; i0 < n; i0 += kThreads / 4) {
+    const int i = i0 + (threadIdx.x >> 2);
+    const uint64_t key = i < n ? s.keys[i] : 0;
     int r = 0;
 #pragma unroll 4
-    for (int j = 0; j < n; ++j) r += s.keys[j] > key ? 1 : 0;
-    if (r < k) s.sorted[r] = key;
+    for (int j = lanes; j < n; j += 4) r += s.keys[j] > key ? 1 : 0;
+    r += __shfl_xor_sync(0xFFFFFFFFu, r, 1);
+    r += __shfl_xor_sync(0xFFFFFFFFu, r, 2);
+    if (i < n && lanes == 0 && r < k) s.sorted[r] = key;
   }
   __syncthreads();
   if (static_cast<int>(threadIdx.x) < min(n, k)) s.keys[threadIdx.x] = s.sorted[threadIdx.x];
@@ -409,7 +451,7 @@ __device__ __forceinline__ void Prune(LongShared& s, int k) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, 4)
     logprobs_long_kernel(const LogprobArgs a, int cluster) {
   using R = Row<T>;
   constexpr int kE = R::kN;
@@ -545,17 +587,22 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
     }
     if (ranks) {
-#pragma unroll
-      for (int u = 0; u < kVectors; ++u) {
-        const int v = v0 + u * kThreads + tid, j = head + v * kE;
-        if (v >= end) continue;
-        const bool before = j + kE <= target;
-        if (before || j > target) {
-          ahead += R::Above(q[u], xt, before);
-        } else {  // the target's vector
+      // Ahead of the target an equal value counts, behind it none; closed
+      // values behind the part's end must not count as equal ones.
+      const int low = head + v0 * kE, high = low + kThreads * kVectors * kE;
+      if (low > target) {
+        ahead += R::template Above<false>(q, xt);
+      } else if (high <= target && high <= head + end * kE) {
+        ahead += R::template Above<true>(q, xt);
+      } else {
+#pragma unroll 1
+        for (int u = 0; u < kVectors; ++u) {
+          const int v = v0 + u * kThreads + tid, j = head + v * kE;
+          if (v >= end) break;
+          const uint4 vector = __ldg(base + v);
 #pragma unroll
           for (int e = 0; e < kE; ++e) {
-            const float x = R::At(q[u], e);
+            const float x = R::At(vector, e);
             ahead += x > xt || (x == xt && j + e < target) ? 1 : 0;
           }
         }
@@ -565,29 +612,26 @@ __global__ void __launch_bounds__(kThreads, 2)
     // The first values take their threshold from the threads' maxima: in each
     // of ceil(k / 4) warps four lanes hold a value of at least the warp's
     // fourth greatest maximum.
+    // Later values lose to an equal earlier one, so they have to be greater.
     float threshold;
-    const bool first = chunk == 0;
-    if (first) {
-      const float fourth = WarpKth(top, 4);
+    if (chunk == 0) {
+      const float fourth = WarpKthOfFew(top, 4);
       if (lane == 0) s.fourth[warp] = fourth;
       __syncthreads();
-      threshold = WarpKth(lane < kThreads / 32 ? s.fourth[lane] : -INFINITY, (k + 3) / 4);
+      threshold = WarpKthOfFew(lane < kThreads / 32 ? s.fourth[lane] : -INFINITY, (k + 3) / 4);
+      if (threshold > -INFINITY) threshold = R::Below(threshold);
     } else {
       threshold = s.threshold;
     }
-    // Later values lose to an equal earlier one, so they have to be greater.
-    auto passes = [&](float x) {
-      return x > threshold || (first && x == threshold && x > -INFINITY);
-    };
-    if (passes(top)) {
+    if (top > threshold) {
 #pragma unroll
       for (int u = 0; u < kVectors; ++u) {
-        if (!passes(R::Top(q[u]))) continue;
+        uint32_t mask = R::MaskAbove(q[u], threshold);
         const int j = head + (v0 + u * kThreads + tid) * kE;
-#pragma unroll
-        for (int e = 0; e < kE; ++e) {
-          const float x = R::At(q[u], e);
-          if (passes(x)) push(x, j + e);
+        while (mask != 0) {
+          const int e = __ffs(mask) - 1;
+          mask &= mask - 1;
+          push(ToFloat(src[j + e]), j + e);
         }
       }
     }
