@@ -475,11 +475,16 @@ __global__ void __launch_bounds__(kThreads, 4)
   const int vectors = (a.vocab - head) / kE;
   const int per = (vectors + cluster - 1) / cluster;
   const int begin = part * per, end = min(vectors, begin + per);
+  constexpr int kStep = kThreads * kVectors;  // vectors of a chunk
   auto load = [&](int v0, uint4 (&q)[kVectors]) {
+    const uint4* p = base + v0 + tid;
+    if (v0 + kStep <= end) {
 #pragma unroll
-    for (int u = 0; u < kVectors; ++u) {
-      const int v = v0 + u * kThreads + tid;
-      q[u] = v < end ? __ldg(base + v) : R::Closed();
+      for (int u = 0; u < kVectors; ++u) q[u] = __ldg(p + u * kThreads);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kVectors; ++u)
+        q[u] = v0 + u * kThreads + tid < end ? __ldg(p + u * kThreads) : R::Closed();
     }
   };
   uint4 next[kVectors];
@@ -562,11 +567,11 @@ __global__ void __launch_bounds__(kThreads, 4)
   }
   int settled = head + begin * kE;  // values below are in order in s.keys
   int chunk = 0;
-  for (int v0 = begin; v0 < end; v0 += kThreads * kVectors, ++chunk) {
+  for (int v0 = begin; v0 < end; v0 += kStep, ++chunk) {
     uint4 q[kVectors];
 #pragma unroll
     for (int u = 0; u < kVectors; ++u) q[u] = next[u];
-    if (v0 + kThreads * kVectors < end) load(v0 + kThreads * kVectors, next);
+    if (v0 + kStep < end) load(v0 + kStep, next);
     const float top = R::Top(q);
     grow(top);
     if (fabsf(st.m) < INFINITY) {
@@ -589,7 +594,7 @@ __global__ void __launch_bounds__(kThreads, 4)
     if (ranks) {
       // Ahead of the target an equal value counts, behind it none; closed
       // values behind the part's end must not count as equal ones.
-      const int low = head + v0 * kE, high = low + kThreads * kVectors * kE;
+      const int low = head + v0 * kE, high = low + kStep * kE;
       if (low > target) {
         ahead += R::template Above<false>(q, xt);
       } else if (high <= target && high <= head + end * kE) {
@@ -637,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, 4)
     }
     // After chunks 1, 2, 4, 8, ...: about top_k values pass in between.
     if ((chunk & (chunk + 1)) == 0) {
-      const int high = head + min(end, v0 + kThreads * kVectors) * kE;
+      const int high = head + min(end, v0 + kStep) * kE;
       settle(settled, high);
       settled = high;
     }
