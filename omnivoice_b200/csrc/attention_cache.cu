@@ -73,8 +73,7 @@ __device__ __forceinline__ void ValueScale(float scale, float* shift, float* inv
 }
 
 // Tokens of a sequence, bounded by what the call announced.
-__device__ __forceinline__ int SequenceLength(const CacheAttnArgs& a, int seq) {
-  const int length = a.lengths[seq];
+__device__ __forceinline__ int CheckLength(const CacheAttnArgs& a, int length) {
   if (length < 0 || length > a.max_length) {
     atomicOr(a.err, kErrBadArgument);
     return length < 0 ? 0 : a.max_length;
@@ -91,12 +90,13 @@ __device__ __forceinline__ int SequenceLength(const CacheAttnArgs& a, int seq) {
 // and the rows its 8-column side.
 //
 // Work is cut into units of 32 keys of one (sequence, kv head), numbered
-// along sequences and heads, and every CTA takes the same count of
-// consecutive units, whatever the lengths.  Each of its 8 warps streams every
-// eighth unit through a ring of its own (TMA, 128B swizzle), with its own
-// running maximum, sums and O; they join in shared memory where the CTA's
-// range leaves a (sequence, head).  One that spans several CTAs is joined by
-// the last of them to arrive, over the parts in CTA order.
+// along heads and sequences, and every warp of the grid takes the same count
+// of consecutive units, whatever the lengths, through a ring of its own (TMA,
+// 128B swizzle).  An item (sequence, kv head) inside one warp's range is
+// stored by it; one that spans warps is joined in shared memory when the
+// CTA's warps are done, one that spans CTAs by the last of them to arrive,
+// always over the parts in order.  When all items fit, each starts at a CTA
+// of its own, which spares most of them the join across CTAs.
 //
 // Fragments straight from the swizzled tiles: lane 4g + c, MMA row g is key
 // kappa(g) of a slab of 16 (and 8 + kappa(g)).  kappa puts neighbouring g
@@ -109,7 +109,7 @@ constexpr int kUnit = 32;               // keys
 constexpr int kUnitTile = kUnit * kCacheHeadDim;  // bytes of K or V of a unit
 constexpr int kStreamWarps = 8;
 constexpr int kStreamThreads = kStreamWarps * 32;
-constexpr int kMinUnits = kStreamWarps;  // of a CTA: one for each warp
+constexpr int kMinUnits = 3;            // of a warp, where items get CTAs of their own
 
 // Ring slot beside the codes: scales and pages of the unit's two 16-key slabs.
 struct alignas(16) SlotInfo {
@@ -120,13 +120,13 @@ struct alignas(16) SlotInfo {
 struct StreamArgs {
   CacheAttnArgs a;
   uint32_t* counters;  // one for each (sequence, kv head); null: no item is split
-  float* parts;        // [CTA][2][JoinFloats(join_rows)]
+  float* parts;        // [CTA][2][JoinFloats(join_rows)]: of the item begun before, of the last
   int join_rows;       // rows of a (sequence, kv head) at most
 };
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                           uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9},"
       " {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -184,25 +184,33 @@ __device__ __forceinline__ void JoinPart(float* top, float* sum, float4* v, floa
   v->w = fmaf(y.w, h, v->w * f);
 }
 
-// Units of a sequence and kv head; one (with nothing to see) where rows need
-// their zeros, none without rows.
-__device__ __forceinline__ int SequenceUnits(const CacheAttnArgs& a, int seq) {
-  const RowSpan span = SequenceRows(a.cu_rows, seq, a.rows, a.max_rows, a.err);
-  if (span.count == 0) return 0;
-  return max(1, (SequenceLength(a, seq) - 1) / kUnit + 1);
-}
-
-// One (sequence, kv head) among the numbered units.
+// One (sequence, kv head).  Its units have numbers begin, begin + 1, ...; the
+// next item's begin `room` behind its own.
 struct ItemAt {
-  int seq, head, units;
-  int64_t begin;  // its first unit's number
+  int seq, head;
+  int first, count, length;  // packed rows, tokens
+  int units, room;
+  int64_t begin;
+
+  // The rows and units of `seq`: one unit (with nothing to see) where rows
+  // need their zeros, none without rows.
+  __device__ __forceinline__ void Load(const CacheAttnArgs& a, int align) {
+    const int from = a.cu_rows[seq], to = a.cu_rows[seq + 1], tokens = a.lengths[seq];
+    const RowSpan span = CheckRows(from, to, a.rows, a.max_rows, a.err);
+    first = span.first;
+    count = span.count;
+    length = CheckLength(a, tokens);
+    units = count == 0 ? 0 : max(1, (length - 1) / kUnit + 1);
+    room = (units + align - 1) / align * align;
+  }
+  __device__ __forceinline__ int64_t end() const { return begin + units; }
   // To the next one that has units; false behind the last.
-  __device__ __forceinline__ bool Next(const CacheAttnArgs& a) {
-    begin += units;
+  __device__ __forceinline__ bool Next(const CacheAttnArgs& a, int align) {
+    begin += room;
     if (++head < a.cache.kv_heads) return true;
     head = 0;
     while (++seq < a.cache.num_seqs) {
-      units = SequenceUnits(a, seq);
+      Load(a, align);
       if (units > 0) return true;
     }
     return false;
@@ -210,16 +218,17 @@ struct ItemAt {
 };
 
 struct alignas(16) StreamShared {
-  int64_t sum[kStreamWarps];
-  ItemAt first;
-  int last;
+  int64_t sum[2][kStreamWarps];
+  ItemAt first[kStreamWarps];  // the item at each warp's first unit; seq -1: none
+  ItemAt part[2];              // items that this CTA shares with others
+  int has[2], last[2];
 };
 
 template <int kNT>
 constexpr int StreamStages() {
   return kNT == 1 ? 3 : 2;
 }
-// Joining buffer of `rows` query rows: O, then maxima and sums, per warp.
+// A part of an item with `rows` query rows: O, then maxima and sums.
 __host__ __device__ constexpr size_t JoinFloats(int rows) {
   return (static_cast<size_t>(rows) * (kCacheHeadDim + 2) + 3) / 4 * 4;
 }
@@ -228,6 +237,28 @@ constexpr size_t StreamSmem(int rows) {
   return 1024 + static_cast<size_t>(StreamStages<kNT>()) * kStreamWarps *
                     (2 * kUnitTile + sizeof(SlotInfo) + sizeof(uint64_t)) +
          sizeof(StreamShared) + kStreamWarps * JoinFloats(rows) * sizeof(float);
+}
+
+// Sum of a value over the block and over the threads before this one; `slot`
+// is a row of sums that no other call uses.
+__device__ __forceinline__ int64_t BlockSum(int64_t mine, int64_t* slot, int64_t* before) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t inclusive = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xFFFFFFFFu, inclusive, o);
+    if (lane >= o) inclusive += v;
+  }
+  if (lane == 31) slot[warp] = inclusive;
+  __syncthreads();
+  int64_t total = 0;
+  *before = inclusive - mine;
+#pragma unroll
+  for (int w = 0; w < kStreamWarps; ++w) {
+    if (w < warp) *before += slot[w];
+    total += slot[w];
+  }
+  return total;
 }
 
 template <int kNT>
@@ -251,7 +282,9 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
                    warp * kStages;
   StreamShared& shared = *reinterpret_cast<StreamShared*>(
       smem + kStreamWarps * kStages * (2 * kUnitTile + sizeof(SlotInfo) + sizeof(uint64_t)));
-  float* join = reinterpret_cast<float*>(&shared + 1);
+  float* join = reinterpret_cast<float*>(&shared + 1);  // [warp][JoinFloats(join_rows)]
+  const size_t join_floats = JoinFloats(args.join_rows);
+  const int stats = args.join_rows * kCacheHeadDim;  // of a part: maxima and sums
   pdl_trigger();
   if (lane == 0) {
     // Lanes 0 and 1 each arrive for their codes and for their scales.
@@ -259,83 +292,111 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     fence_mbar_init();
     tma_prefetch_map(&map_k);
     tma_prefetch_map(&map_v);
+    shared.first[warp].seq = -1;
+    if (warp == 0) shared.has[0] = shared.has[1] = 0;
   }
   pdl_wait();
 
-  // This CTA's units [b0, b1) and the item that holds the first.
-  int64_t b0, b1, share = 0;
-  if (args.counters == nullptr) {
-    if (tid == 0) {
-      shared.first.seq = static_cast<int>(blockIdx.x) / cache.kv_heads;
-      shared.first.head = static_cast<int>(blockIdx.x) % cache.kv_heads;
-      shared.first.units = SequenceUnits(a, shared.first.seq);
-      shared.first.begin = 0;
-    }
+  // This warp's numbers [p0, p1), of the CTA's from `base` on, and the item at p0.
+  int align = 1;
+  int64_t width;  // numbers of a warp
+  int64_t base;
+  int own_units = 0;
+  if (args.counters == nullptr) {  // the CTA has an item to itself
+    ItemAt item;
+    item.seq = static_cast<int>(blockIdx.x) / cache.kv_heads;
+    item.head = static_cast<int>(blockIdx.x) % cache.kv_heads;
+    item.begin = 0;
+    item.Load(a, 1);
+    width = (item.units + kStreamWarps - 1) / kStreamWarps;
+    base = 0;
+    own_units = item.units;
+    if (item.units == 0) return;  // uniform over the CTA
     __syncthreads();
-    b0 = 0;
-    b1 = shared.first.units;
+    if (tid < kStreamWarps && tid * width < item.units) shared.first[tid] = item;
+    __syncthreads();
   } else {
     const int per = (cache.num_seqs + kStreamThreads - 1) / kStreamThreads;
     const int first = min(cache.num_seqs, tid * per), last = min(cache.num_seqs, first + per);
-    int64_t mine = 0;
-    for (int s = first; s < last; ++s) mine += SequenceUnits(a, s);
+    ItemAt item;
+    int64_t mine = 0, before;
+    for (item.seq = first; item.seq < last; ++item.seq) {
+      item.Load(a, 1);
+      mine += item.units;
+    }
+    const int64_t units = BlockSum(mine, shared.sum[0], &before) * cache.kv_heads;
+    width = (units + gridDim.x * kStreamWarps - 1) / (gridDim.x * kStreamWarps);
+    // CTAs that the items would take with a begin of their own.
+    const int wide = static_cast<int>(max(width, static_cast<int64_t>(kMinUnits))) * kStreamWarps;
+    int64_t ctas = 0;
+    if (per == 1) {
+      if (first < last) ctas = (item.units + wide - 1) / wide;
+    } else {
+      for (item.seq = first; item.seq < last; ++item.seq) {
+        item.Load(a, wide);
+        ctas += item.room / wide;
+      }
+    }
+    int64_t ctas_before;
+    const int64_t all = BlockSum(ctas, shared.sum[1], &ctas_before) * cache.kv_heads;
+    if (all <= gridDim.x) {
+      align = wide;
+      width = wide / kStreamWarps;
+      mine = ctas * align;
+      before = ctas_before * align;
+    }
     mine *= cache.kv_heads;
-    int64_t inclusive = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xFFFFFFFFu, inclusive, o);
-      if (lane >= o) inclusive += v;
-    }
-    if (lane == 31) shared.sum[warp] = inclusive;
-    __syncthreads();
-    int64_t total = 0, before = inclusive - mine;
-#pragma unroll
-    for (int w = 0; w < kStreamWarps; ++w) {
-      if (w < warp) before += shared.sum[w];
-      total += shared.sum[w];
-    }
-    share = max(static_cast<int64_t>(kMinUnits), (total + gridDim.x - 1) / gridDim.x);
-    b0 = share * blockIdx.x;
-    b1 = min(total, b0 + share);
-    if (before <= b0 && b0 < before + mine) {
+    before *= cache.kv_heads;
+    base = width * kStreamWarps * blockIdx.x;
+    if (base < before + mine && before < base + width * kStreamWarps) {
+      // Some warps of the CTA begin in this thread's sequences.
       for (int s = first; s < last; ++s) {
-        const int units = SequenceUnits(a, s);
-        const int64_t all = static_cast<int64_t>(units) * cache.kv_heads;
-        if (b0 < before + all) {
-          const int head = static_cast<int>((b0 - before) / units);
-          shared.first = {s, head, units, before + static_cast<int64_t>(head) * units};
-          break;
+        item.seq = s;
+        if (per > 1) item.Load(a, align);
+        else item.room = (item.units + align - 1) / align * align;
+        const int64_t span = static_cast<int64_t>(item.room) * cache.kv_heads;
+        for (int w = 0; w < kStreamWarps; ++w) {
+          const int64_t p = base + w * width;
+          if (p < before || p >= before + span) continue;
+          item.head = static_cast<int>((p - before) / item.room);
+          item.begin = before + static_cast<int64_t>(item.head) * item.room;
+          shared.first[w] = item;
         }
-        before += all;
+        before += span;
       }
     }
     __syncthreads();
   }
-  if (b0 >= b1) return;
-  __syncwarp();
+  // Without counters a CTA's numbers end with its item, else its last warps
+  // would go on to the next one, which is another CTA's.
+  const int64_t p0 = base + warp * width;
+  const int64_t p1 = args.counters == nullptr ? min(p0 + width, static_cast<int64_t>(own_units))
+                                              : p0 + width;
+  ItemAt item = shared.first[warp];
 
-  // The unit to load next (this warp's position q0) and its pages, one ahead.
-  ItemAt fetch = shared.first;
-  int64_t fetch_at = b0 + warp;
-  int fetch_page = -1;   // lanes 0 and 1: page of slab `lane`
-  int fetch_length = 0;
-  bool fetch_slot = false;  // whether this lane has a page to ask for
-  auto look_up = [&] {  // the page of this lane's slab of unit fetch_at
-    while (fetch_at < b1 && fetch_at >= fetch.begin + fetch.units) {
-      if (!fetch.Next(a)) break;
+  // The unit to load next, and the page of this lane's slab (lanes 0 and 1).
+  ItemAt fetch = item;
+  int64_t fetch_at = item.seq < 0 ? p1 : p0;
+  int fetch_page = -1;
+  bool fetch_slot = false;  // whether this lane's slab has tokens
+  auto look_up = [&] {
+    while (fetch_at < p1 && fetch_at >= fetch.end()) {
+      if (!fetch.Next(a, align)) {
+        fetch_at = p1;
+        break;
+      }
+      fetch_at = fetch.begin;
     }
-    if (fetch_at >= b1) return;
-    fetch_length = SequenceLength(a, fetch.seq);
-    const int token = static_cast<int>(fetch_at - fetch.begin) * kUnit;
-    const int mine = token + (lane & 1) * 16;
-    fetch_slot = lane < 2 && mine < fetch_length;
+    if (fetch_at >= p1) return;
+    const int token = static_cast<int>(fetch_at - fetch.begin) * kUnit + (lane & 1) * 16;
+    fetch_slot = lane < 2 && token < fetch.length;
     if (fetch_slot)
       fetch_page = cache.table[static_cast<int64_t>(fetch.seq) * cache.max_pages +
-                               (mine >> cache.page_shift)];
+                               (token >> cache.page_shift)];
   };
   const int box = min(kUnit, 1 << cache.page_shift);  // rows of a TMA box
   auto issue = [&](int stage) {
-    if (fetch_at >= b1) return;
+    if (fetch_at >= p1) return;
     if (lane < 2) {
       uint64_t* bar = &full[stage];
       int page = fetch_slot ? fetch_page : -1;
@@ -351,8 +412,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
       } else {
         info[stage].scale[2 * lane] = info[stage].scale[2 * lane + 1] = 1.0f;
       }
-      const bool loads = page >= 0 && (lane == 0 || box < kUnit);
-      if (loads) {
+      if (page >= 0 && (lane == 0 || box < kUnit)) {
         const int token = static_cast<int>(fetch_at - fetch.begin) * kUnit + lane * 16;
         const int row = ((page * cache.kv_heads + fetch.head) << cache.page_shift) +
                         (token & ((1 << cache.page_shift) - 1));
@@ -365,7 +425,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
       }
       cp_async_arrive(bar);
     }
-    fetch_at += kStreamWarps;
+    ++fetch_at;
     look_up();
   };
   look_up();
@@ -384,36 +444,26 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     const int key = key_c + (later != (j == 1) ? 4 : 0);
     v_at[j] = key * kCacheHeadDim + ((g ^ key) << 4);
   }
+  // Where row r of an item is stored.
+  auto out_row = [&](const ItemAt& it, int r) {
+    const int token = a.group(r);
+    return a.out + static_cast<int64_t>(it.first + token) * a.ld_out +
+           (it.head * a.group.d + r - token * a.group.d) * kCacheHeadDim;
+  };
 
-  ItemAt item = shared.first;
-  int64_t at = b0 + warp;
+  int64_t at = p0;
   int done = 0;  // units of this warp so far
   bool ok = true;  // once a wait ran out, no other is begun
-  while (true) {
-    const int64_t item_end = item.begin + item.units;
-    const int64_t end = min(b1, item_end);
-    const RowSpan span = SequenceRows(a.cu_rows, item.seq, a.rows, a.max_rows, a.err);
-    const int length = SequenceLength(a, item.seq);
-    const int rows = span.count * a.group.d;  // row r: token r / group, head r % group
-    float m[kNT][2], l[kNT][2], o[8][kNT][4];
-    int seen[kNT][2];  // tokens that column 2c + e sees
-    uint32_t q[2][4][kNT][2];
-    const int least = a.causal ? length - span.count + 1 : length;
-#pragma unroll
-    for (int t = 0; t < kNT; ++t) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        m[t][e] = -INFINITY;
-        l[t][e] = 0.0f;
-        const int r = t * 8 + 2 * c + e;
-        seen[t][e] = a.causal && r < rows ? least + a.group(r) : length;
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][t][e] = 0.0f;
-    }
+  bool tail = false;  // `item` goes on behind p1 and began here
+  while (item.seq >= 0 && at < p1) {
+    const int64_t end = min(p1, item.end());
     if (at < end) {
+      const int rows = item.count * a.group.d;  // row r: token r / group, head r % group
+      const bool begun = at == item.begin;
+      float m[kNT][2], l[kNT][2], o[8][kNT][4];
+      int seen[kNT][2];  // tokens that column 2c + e sees
+      uint32_t q[2][4][kNT][2];
+      const int least = a.causal ? item.length - item.count + 1 : item.length;
 #pragma unroll
       for (int t = 0; t < kNT; ++t) {
         const int r = t * 8 + g;
@@ -421,7 +471,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
         const __half* src = a.q;
         if (live) {
           const int token = a.group(r);
-          src += static_cast<int64_t>(span.first + token) * a.ld_q +
+          src += static_cast<int64_t>(item.first + token) * a.ld_q +
                  (item.head * a.group.d + r - token * a.group.d) * kCacheHeadDim + 16 * c;
         }
 #pragma unroll
@@ -436,224 +486,258 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
           q[j][2][t][0] = y.x, q[j][2][t][1] = y.y;
           q[j][3][t][0] = y.z, q[j][3][t][1] = y.w;
         }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          m[t][e] = -INFINITY;
+          l[t][e] = 0.0f;
+          const int column = t * 8 + 2 * c + e;
+          seen[t][e] = a.causal && column < rows ? least + a.group(column) : item.length;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i][t][e] = 0.0f;
       }
-    }
-    for (; at < end; at += kStreamWarps) {
-      const int stage = done % kStages;
-      ok = ok && mbar_wait(&full[stage], static_cast<uint32_t>(done / kStages) & 1u, a.err);
-      __syncwarp();
-      const uint8_t* keys = ring + stage * 2 * kUnitTile;
-      const uint8_t* values = keys + kUnitTile;
-      const int token0 = static_cast<int>(at - item.begin) * kUnit;
-      float s[2][kNT][4], shift[2], inverse[2];
-      const float4 scales = *reinterpret_cast<const float4*>(info[stage].scale);
-      const int2 pages = *reinterpret_cast<const int2*>(info[stage].page);
-      const float factor[2] = {KeyFactor(scales.x, a.scale_log2), KeyFactor(scales.z, a.scale_log2)};
-      ValueScale(scales.y, &shift[0], &inverse[0]);
-      ValueScale(scales.w, &shift[1], &inverse[1]);
+      for (; at < end; ++at) {
+        const int stage = done % kStages;
+        ok = ok && mbar_wait(&full[stage], static_cast<uint32_t>(done / kStages) & 1u, a.err);
+        __syncwarp();
+        const uint8_t* keys = ring + stage * 2 * kUnitTile;
+        const uint8_t* values = keys + kUnitTile;
+        const int token0 = static_cast<int>(at - item.begin) * kUnit;
+        float s[2][kNT][4], shift[2], inverse[2];
+        const float4 scales = *reinterpret_cast<const float4*>(info[stage].scale);
+        const int2 pages = *reinterpret_cast<const int2*>(info[stage].page);
+        const float factor[2] = {KeyFactor(scales.x, a.scale_log2), KeyFactor(scales.z, a.scale_log2)};
+        ValueScale(scales.y, &shift[0], &inverse[0]);
+        ValueScale(scales.w, &shift[1], &inverse[1]);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int t = 0; t < kNT; ++t) s[h][t][0] = s[h][t][1] = s[h][t][2] = s[h][t][3] = 0.0f;
+          for (int t = 0; t < kNT; ++t) s[h][t][0] = s[h][t][1] = s[h][t][2] = s[h][t][3] = 0.0f;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const uint8_t* p = keys + h * 16 * kCacheHeadDim + k_at[j];
-          const uint4 x = *reinterpret_cast<const uint4*>(p);
-          const uint4 y = *reinterpret_cast<const uint4*>(p + 8 * kCacheHeadDim);
-          const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+          uint32_t x[2][2][4];  // slab, keys of rows g and g + 8
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const uint32_t u = xs[r] ^ 0x80808080u, v = ys[r] ^ 0x80808080u;
-            const uint32_t f[4] = {CodePair<0x4140>(u), CodePair<0x4140>(v), CodePair<0x4342>(u),
-                                   CodePair<0x4342>(v)};
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int t = 0; t < kNT; ++t) mma_16816(s[h][t], f, q[j][r][t][0], q[j][r][t][1]);
-          }
-        }
-      }
-      // Exponents, then the maximum, raised only when one passes it by 2^8.
-      const bool partial = token0 + kUnit > least || pages.x < 0 || pages.y < 0;
-      bool grow = false;
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int t = 0; t < kNT; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float& v = s[h][t][e];
-            v = fmaf(v, factor[h], shift[h]);
-            if (partial) {
-              const int key = token0 + h * 16 + key_g + (e >> 1) * 8;
-              if (key >= seen[t][e & 1] || (h == 0 ? pages.x : pages.y) < 0) v = -INFINITY;
+            for (int i = 0; i < 2; ++i) {
+              const uint4 v = *reinterpret_cast<const uint4*>(keys + (h * 16 + i * 8) * kCacheHeadDim + k_at[j]);
+              x[h][i][0] = v.x ^ 0x80808080u;
+              x[h][i][1] = v.y ^ 0x80808080u;
+              x[h][i][2] = v.z ^ 0x80808080u;
+              x[h][i][3] = v.w ^ 0x80808080u;
             }
-            grow |= v > m[t][e & 1] + 8.0f;
-          }
-      if (__any_sync(0xFFFFFFFFu, grow)) {
 #pragma unroll
-        for (int t = 0; t < kNT; ++t)
+          for (int r = 0; r < 4; ++r)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float top = fmaxf(fmaxf(s[0][t][e], s[0][t][e + 2]), fmaxf(s[1][t][e], s[1][t][e + 2]));
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
-            if (top > m[t][e]) {
-              const float old = ex2_approx(m[t][e] - top);
-              m[t][e] = top;
-              l[t][e] *= old;
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t f[4] = {CodePair<0x4140>(x[h][0][r]), CodePair<0x4140>(x[h][1][r]),
+                                     CodePair<0x4342>(x[h][0][r]), CodePair<0x4342>(x[h][1][r])};
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                o[i][t][e] *= old;
-                o[i][t][e + 2] *= old;
+              for (int t = 0; t < kNT; ++t) mma_16816(s[h][t], f, q[j][r][t][0], q[j][r][t][1]);
+            }
+        }
+        // Exponents, then the maximum, raised only when one passes it by 2^8.
+        const bool partial = token0 + kUnit > least || pages.x < 0 || pages.y < 0;
+        bool grow = false;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int t = 0; t < kNT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float& v = s[h][t][e];
+              v = fmaf(v, factor[h], shift[h]);
+              if (partial) {
+                const int key = token0 + h * 16 + key_g + (e >> 1) * 8;
+                if (key >= seen[t][e & 1] || (h == 0 ? pages.x : pages.y) < 0) v = -INFINITY;
+              }
+              grow |= v > m[t][e & 1] + 8.0f;
+            }
+        if (__any_sync(0xFFFFFFFFu, grow)) {
+#pragma unroll
+          for (int t = 0; t < kNT; ++t)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float top = fmaxf(fmaxf(s[0][t][e], s[0][t][e + 2]), fmaxf(s[1][t][e], s[1][t][e + 2]));
+              top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
+              top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
+              top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
+              if (top > m[t][e]) {
+                const float old = ex2_approx(m[t][e] - top);
+                m[t][e] = top;
+                l[t][e] *= old;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  o[i][t][e] *= old;
+                  o[i][t][e + 2] *= old;
+                }
               }
             }
-          }
-      }
-      uint32_t pb[2][kNT][2];
+        }
+        uint32_t pb[2][kNT][2];
 #pragma unroll
-      for (int t = 0; t < kNT; ++t) {
-        const float m0 = m[t][0] == -INFINITY ? 0.0f : m[t][0];
-        const float m1 = m[t][1] == -INFINITY ? 0.0f : m[t][1];
+        for (int t = 0; t < kNT; ++t) {
+          const float m0 = m[t][0] == -INFINITY ? 0.0f : m[t][0];
+          const float m1 = m[t][1] == -INFINITY ? 0.0f : m[t][1];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float e0 = ex2_approx(s[h][t][0] - m0), e1 = ex2_approx(s[h][t][1] - m1);
+            const float e2 = ex2_approx(s[h][t][2] - m0), e3 = ex2_approx(s[h][t][3] - m1);
+            l[t][0] = fmaf(e0 + e2, inverse[h], l[t][0]);
+            l[t][1] = fmaf(e1 + e3, inverse[h], l[t][1]);
+            pb[h][t][0] = transpose_8x8(pack_half2(e0, e1));
+            pb[h][t][1] = transpose_8x8(pack_half2(e2, e3));
+          }
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float p0 = ex2_approx(s[h][t][0] - m0), p1 = ex2_approx(s[h][t][1] - m1);
-          const float p2 = ex2_approx(s[h][t][2] - m0), p3 = ex2_approx(s[h][t][3] - m1);
-          l[t][0] = fmaf(p0 + p2, inverse[h], l[t][0]);
-          l[t][1] = fmaf(p1 + p3, inverse[h], l[t][1]);
-          pb[h][t][0] = transpose_8x8(pack_half2(p0, p1));
-          pb[h][t][1] = transpose_8x8(pack_half2(p2, p3));
-        }
-      }
+          const uint8_t* p = values + h * 16 * kCacheHeadDim;
+          const uint4 x0 = *reinterpret_cast<const uint4*>(p + v_at[0]);
+          const uint4 x1 = *reinterpret_cast<const uint4*>(p + v_at[1]);
+          const uint4 x2 = *reinterpret_cast<const uint4*>(p + v_at[0] + 8 * kCacheHeadDim);
+          const uint4 x3 = *reinterpret_cast<const uint4*>(p + v_at[1] + 8 * kCacheHeadDim);
+          const uint32_t w0[4] = {x0.x, x0.y, x0.z, x0.w}, w1[4] = {x1.x, x1.y, x1.z, x1.w};
+          const uint32_t w2[4] = {x2.x, x2.y, x2.z, x2.w}, w3[4] = {x3.x, x3.y, x3.z, x3.w};
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint8_t* p = values + h * 16 * kCacheHeadDim;
-        const uint4 x0 = *reinterpret_cast<const uint4*>(p + v_at[0]);
-        const uint4 x1 = *reinterpret_cast<const uint4*>(p + v_at[1]);
-        const uint4 x2 = *reinterpret_cast<const uint4*>(p + v_at[0] + 8 * kCacheHeadDim);
-        const uint4 x3 = *reinterpret_cast<const uint4*>(p + v_at[1] + 8 * kCacheHeadDim);
-        const uint32_t w0[4] = {x0.x, x0.y, x0.z, x0.w}, w1[4] = {x1.x, x1.y, x1.z, x1.w};
-        const uint32_t w2[4] = {x2.x, x2.y, x2.z, x2.w}, w3[4] = {x3.x, x3.y, x3.z, x3.w};
+          for (int r = 0; r < 4; ++r) {
+            const uint32_t u0 = w0[r] ^ 0x80808080u, u1 = w1[r] ^ 0x80808080u;
+            const uint32_t u2 = w2[r] ^ 0x80808080u, u3 = w3[r] ^ 0x80808080u;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const uint32_t u0 = w0[r] ^ 0x80808080u, u1 = w1[r] ^ 0x80808080u;
-          const uint32_t u2 = w2[r] ^ 0x80808080u, u3 = w3[r] ^ 0x80808080u;
+            for (int b = 0; b < 2; ++b) {  // dims 16 g + 4 r + 2 b, and one more
+              const uint32_t sel = b == 0 ? pair_lo : pair_hi;
+              const uint32_t near = __byte_perm(u0, u1, sel), far = __byte_perm(u2, u3, sel);
+              const uint32_t f[4] = {CodePair<0x4140>(near), CodePair<0x4342>(near),
+                                     CodePair<0x4140>(far), CodePair<0x4342>(far)};
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {  // dims 16 g + 4 r + 2 b, and one more
-            const uint32_t sel = b == 0 ? pair_lo : pair_hi;
-            const uint32_t near = __byte_perm(u0, u1, sel), far = __byte_perm(u2, u3, sel);
-            const uint32_t f[4] = {CodePair<0x4140>(near), CodePair<0x4342>(near),
-                                   CodePair<0x4140>(far), CodePair<0x4342>(far)};
-#pragma unroll
-            for (int t = 0; t < kNT; ++t) mma_16816(o[2 * r + b][t], f, pb[h][t][0], pb[h][t][1]);
+              for (int t = 0; t < kNT; ++t) mma_16816(o[2 * r + b][t], f, pb[h][t][0], pb[h][t][1]);
+            }
           }
         }
+        ++done;
+        __syncwarp();
+        issue(stage);
       }
-      ++done;
-      __syncwarp();
-      issue(stage);
-    }
 
-    // Join the warps' parts: O[row][128], then (maximum, sum) of each row.
-    float* part = join + warp * JoinFloats(args.join_rows);
+      // Out, or a part: of an item begun before p0 in `join`, of one that goes
+      // on behind p1 in this warp's ring, which is idle by then.
+      const bool whole = begun && end == item.end();
+      tail = begun && !whole;
+      float* part = tail ? reinterpret_cast<float*>(ring) : join + warp * join_floats;
 #pragma unroll
-    for (int t = 0; t < kNT; ++t)
+      for (int t = 0; t < kNT; ++t)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float sum = l[t][e];
-        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 4);
-        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 8);
-        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 16);
-        const int r = t * 8 + 2 * c + e;
-        if (r < rows) {
-          float4* dst = reinterpret_cast<float4*>(part + r * kCacheHeadDim + 16 * g);
+        for (int e = 0; e < 2; ++e) {
+          float sum = l[t][e];
+          sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 4);
+          sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 8);
+          sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 16);
+          const int r = t * 8 + 2 * c + e;
+          if (r >= rows) continue;
+          if (whole) {
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            uint4* dst = reinterpret_cast<uint4*>(out_row(item, r) + 16 * g);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            dst[i] = make_float4(o[2 * i][t][e], o[2 * i][t][e + 2], o[2 * i + 1][t][e],
-                                 o[2 * i + 1][t][e + 2]);
-          if (g == 0) {
-            part[args.join_rows * kCacheHeadDim + 2 * r] = m[t][e];
-            part[args.join_rows * kCacheHeadDim + 2 * r + 1] = sum;
+            for (int i = 0; i < 2; ++i)
+              dst[i] = make_uint4(pack_half2(o[4 * i][t][e] * inv, o[4 * i][t][e + 2] * inv),
+                                  pack_half2(o[4 * i + 1][t][e] * inv, o[4 * i + 1][t][e + 2] * inv),
+                                  pack_half2(o[4 * i + 2][t][e] * inv, o[4 * i + 2][t][e + 2] * inv),
+                                  pack_half2(o[4 * i + 3][t][e] * inv, o[4 * i + 3][t][e + 2] * inv));
+          } else {
+            float4* dst = reinterpret_cast<float4*>(part + r * kCacheHeadDim + 16 * g);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              dst[i] = make_float4(o[2 * i][t][e], o[2 * i][t][e + 2], o[2 * i + 1][t][e],
+                                   o[2 * i + 1][t][e + 2]);
+            if (g == 0)
+              *reinterpret_cast<float2*>(part + stats + 2 * r) = make_float2(m[t][e], sum);
           }
         }
-      }
-    __syncthreads();
-    const bool whole = item.begin >= b0 && item_end <= b1;
-    const int stats = args.join_rows * kCacheHeadDim;
-    auto store_row = [&](int r, int d, float4 v, float sum) {
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      const int token = a.group(r);
-      __half* dst = a.out + static_cast<int64_t>(span.first + token) * a.ld_out +
-                    (item.head * a.group.d + r - token * a.group.d) * kCacheHeadDim + d;
-      *reinterpret_cast<uint2*>(dst) =
-          make_uint2(pack_half2(v.x * inv, v.y * inv), pack_half2(v.z * inv, v.w * inv));
-    };
-    float* slot = whole ? nullptr
-                        : args.parts + (static_cast<int64_t>(blockIdx.x) * 2 +
-                                        (item.begin < b0 ? 0 : 1)) *
-                                           JoinFloats(args.join_rows);
-    for (int i = tid; i < rows * (kCacheHeadDim / 4); i += kStreamThreads) {
-      const int r = i / (kCacheHeadDim / 4), d = i % (kCacheHeadDim / 4) * 4;
-      float top = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kStreamWarps; ++w)
-        top = fmaxf(top, join[w * JoinFloats(args.join_rows) + stats + 2 * r]);
-      const float base = top == -INFINITY ? 0.0f : top;
+    }
+    at = min(p1, item.begin + item.room);
+    if (at >= p1 || !item.Next(a, align)) break;
+  }
+  __syncthreads();
+
+  // Joins: an item is the work of the warp that begins it (warp 0 also has
+  // the one begun before the CTA).
+  const int64_t cta_end = base + width * kStreamWarps;
+  auto store_vector = [&](const ItemAt& it, int r, int d, float4 v, float sum) {
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    *reinterpret_cast<uint2*>(out_row(it, r) + d) =
+        make_uint2(pack_half2(v.x * inv, v.y * inv), pack_half2(v.z * inv, v.w * inv));
+  };
+  auto join_warps = [&](const ItemAt& it, bool begun) {
+    const int last = static_cast<int>(min(static_cast<int64_t>(kStreamWarps),
+                                          (it.end() - 1 - base) / width + 1));
+    const int slot = begun ? 1 : 0;
+    const bool whole = begun && it.end() <= cta_end;
+    float* dst = whole ? nullptr : args.parts + (static_cast<int64_t>(blockIdx.x) * 2 + slot) * join_floats;
+    const int d = lane * 4;
+    for (int r = 0; r < it.count * a.group.d; ++r) {
+      float top = -INFINITY, sum = 0.0f;
       float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      float sum = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kStreamWarps; ++w) {
-        const float* p = join + w * JoinFloats(args.join_rows);
-        const float f = ex2_approx(p[stats + 2 * r] - base);
-        const float4 x = *reinterpret_cast<const float4*>(p + r * kCacheHeadDim + d);
-        v.x = fmaf(x.x, f, v.x);
-        v.y = fmaf(x.y, f, v.y);
-        v.z = fmaf(x.z, f, v.z);
-        v.w = fmaf(x.w, f, v.w);
-        sum = fmaf(p[stats + 2 * r + 1], f, sum);
+#pragma unroll 4
+      for (int w = warp; w < last; ++w) {
+        const float* p = w == warp && begun ? reinterpret_cast<const float*>(ring) : join + w * join_floats;
+        JoinPart(&top, &sum, &v, *reinterpret_cast<const float2*>(p + stats + 2 * r),
+                 *reinterpret_cast<const float4*>(p + r * kCacheHeadDim + d));
       }
       if (whole) {
-        store_row(r, d, v, sum);
+        store_vector(it, r, d, v, sum);
       } else {
-        *reinterpret_cast<float4*>(slot + r * kCacheHeadDim + d) = v;
-        if (d == 0) *reinterpret_cast<float2*>(slot + stats + 2 * r) = make_float2(top, sum);
-        __threadfence();
+        *reinterpret_cast<float4*>(dst + r * kCacheHeadDim + d) = v;
+        if (lane == 0) *reinterpret_cast<float2*>(dst + stats + 2 * r) = make_float2(top, sum);
       }
     }
-    __syncthreads();
-    if (!whole) {
-      // The last CTA of the item to arrive joins its parts, in CTA order.
-      const int first = static_cast<int>(item.begin / share);
-      const int last = static_cast<int>((item_end - 1) / share);
-      uint32_t* counter = args.counters + static_cast<int64_t>(item.seq) * cache.kv_heads + item.head;
-      if (tid == 0) {
-        __threadfence();
-        shared.last = atomicAdd(counter, 1u) == static_cast<uint32_t>(last - first);
-        if (shared.last) *counter = 0;
-      }
-      __syncthreads();
-      if (shared.last) {
-        __threadfence();
-        for (int i = tid; i < rows * (kCacheHeadDim / 4); i += kStreamThreads) {
-          const int r = i / (kCacheHeadDim / 4), d = i % (kCacheHeadDim / 4) * 4;
-          float top = -INFINITY, sum = 0.0f;
-          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-          for (int x = first; x <= last; ++x) {
-            const float* p = args.parts + (static_cast<int64_t>(x) * 2 +
-                                           (item.begin < x * share ? 0 : 1)) *
-                                              JoinFloats(args.join_rows);
-            const float2 ms = __ldcg(reinterpret_cast<const float2*>(p + stats + 2 * r));
-            const float4 y = __ldcg(reinterpret_cast<const float4*>(p + r * kCacheHeadDim + d));
-            JoinPart(&top, &sum, &v, ms, y);
-          }
-          store_row(r, d, v, sum);
-        }
-      }
-      __syncthreads();
+    if (!whole && lane == 0) {
+      shared.part[slot] = it;
+      shared.has[slot] = 1;
     }
-    if (item_end >= b1 || !item.Next(a)) break;
+  };
+  if (warp == 0) {
+    const ItemAt it = shared.first[0];
+    if (it.seq >= 0 && it.begin < base && base < it.end()) join_warps(it, false);
+  }
+  if (tail) join_warps(item, true);
+  __syncthreads();
+
+  // The last CTA of an item to arrive joins its parts, in CTA order.
+  if (shared.has[0] + shared.has[1] == 0) return;
+  const int64_t cta_width = width * kStreamWarps;
+  if (tid < 2 && shared.has[tid] != 0) {
+    const ItemAt it = shared.part[tid];
+    const int64_t parts = (it.end() - 1) / cta_width - it.begin / cta_width;
+    uint32_t* counter = args.counters + static_cast<int64_t>(it.seq) * cache.kv_heads + it.head;
+    __threadfence();
+    const bool last = atomicAdd(counter, 1u) == static_cast<uint32_t>(parts);
+    if (last) *counter = 0;
+    __threadfence();
+    shared.last[tid] = last;
+  }
+  __syncthreads();
+  for (int slot = 0; slot < 2; ++slot) {
+    if (shared.has[slot] == 0 || shared.last[slot] == 0) continue;
+    const ItemAt it = shared.part[slot];
+    const int first = static_cast<int>(it.begin / cta_width);
+    const int last = static_cast<int>((it.end() - 1) / cta_width);
+    for (int i = tid; i < it.count * a.group.d * (kCacheHeadDim / 4); i += kStreamThreads) {
+      const int r = i / (kCacheHeadDim / 4), d = i % (kCacheHeadDim / 4) * 4;
+      float top = -INFINITY, sum = 0.0f;
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+      for (int x = first; x <= last; ++x) {
+        // The first CTA began the item: its part is its second, the others' their first.
+        const float* p = args.parts + (static_cast<int64_t>(x) * 2 + (x == first ? 1 : 0)) * join_floats;
+        const float2 ms = __ldcg(reinterpret_cast<const float2*>(p + stats + 2 * r));
+        JoinPart(&top, &sum, &v, ms, __ldcg(reinterpret_cast<const float4*>(p + r * kCacheHeadDim + d)));
+      }
+      store_vector(it, r, d, v, sum);
+    }
   }
 }
+
 // ---------------------------------------- many rows: tiles on tcgen05
 //
 // The rows of a kv head (row r: token r / group, head r % group) in tiles of
@@ -865,7 +949,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const int rows = span.count * a.group.d;  // at most 2^31 (host check)
   const int row0 = tile * args.tile_rows;
   if (row0 >= rows) return;  // uniform over the CTA, before any barrier
-  const int length = SequenceLength(a, seq);
+  const int length = CheckLength(a, a.lengths[seq]);
   const bool pair = rows - row0 > kQ && args.tile_rows > kQ;
   const int here = min(rows - row0, args.tile_rows);
   const int last_token = a.group(row0 + here - 1);
@@ -1295,9 +1379,10 @@ StreamPlan PlanStream(const ov_kv_cache* cache, size_t max_rows, size_t max_leng
   if (rows > 16) return plan;
   plan.rows = static_cast<int>(rows);
   const size_t items = cache->num_seqs * cache->kv_heads;
-  const size_t units = items * std::max<size_t>(1, (max_length + kUnit - 1) / kUnit);
+  const size_t units = std::max<size_t>(1, (max_length + kUnit - 1) / kUnit);
+  const size_t least = kMinUnits * kStreamWarps;
   plan.ctas = static_cast<unsigned>(
-      std::min<size_t>(SmCount(), (units + kMinUnits - 1) / kMinUnits));
+      std::min<size_t>(SmCount(), items * ((units + least - 1) / least)));
   plan.counter_bytes = (items * sizeof(uint32_t) + 15) / 16 * 16;
   plan.part_bytes = 2 * plan.ctas * JoinFloats(plan.rows) * sizeof(float);
   return plan;

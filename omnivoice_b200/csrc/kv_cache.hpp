@@ -69,15 +69,19 @@ struct RowSpan {
   int count;
 };
 
-// Packed rows of a sequence; none (reported) when its bounds are not valid.
-__device__ __forceinline__ RowSpan SequenceRows(const int32_t* cu_rows, int seq, int rows,
-                                                int max_rows, uint32_t* err) {
-  const int begin = cu_rows[seq], end = cu_rows[seq + 1];
+// Packed rows [begin, end) of a sequence; none (reported) when its bounds are
+// not valid.
+__device__ __forceinline__ RowSpan CheckRows(int begin, int end, int rows, int max_rows,
+                                             uint32_t* err) {
   if (begin < 0 || end < begin || end > rows || end - begin > max_rows) {
     atomicOr(err, kErrBadArgument);
     return {0, 0};
   }
   return {begin, end - begin};
+}
+__device__ __forceinline__ RowSpan SequenceRows(const int32_t* cu_rows, int seq, int rows,
+                                                int max_rows, uint32_t* err) {
+  return CheckRows(cu_rows[seq], cu_rows[seq + 1], rows, max_rows, err);
 }
 
 #endif  // __CUDACC__
