@@ -92,7 +92,8 @@ __device__ __forceinline__ int CheckLength(const CacheAttnArgs& a, int length) {
 // Work is cut into units of 32 keys of one (sequence, kv head), numbered
 // along heads and sequences, and every warp of the grid takes the same count
 // of consecutive units, whatever the lengths, through a ring of its own (TMA,
-// 128B swizzle).  An item (sequence, kv head) inside one warp's range is
+// 128B swizzle) that a producer warp fills for it (a lane each for two warps:
+// issuing a TMA load takes a warp about a hundred cycles).  An item (sequence, kv head) inside one warp's range is
 // stored by it; one that spans warps is joined in shared memory when the
 // CTA's warps are done, one that spans CTAs by the last of them to arrive,
 // always over the parts in order.  When all items fit, each starts at a CTA
@@ -108,13 +109,15 @@ __device__ __forceinline__ int CheckLength(const CacheAttnArgs& a, int length) {
 constexpr int kUnit = 32;               // keys
 constexpr int kUnitTile = kUnit * kCacheHeadDim;  // bytes of K or V of a unit
 constexpr int kStreamWarps = 8;
-constexpr int kStreamThreads = kStreamWarps * 32;
+constexpr int kStreamThreads = kStreamWarps * 32;  // of the warps that compute
 constexpr int kMinUnits = 3;            // of a warp, where items get CTAs of their own
 
-// Ring slot beside the codes: scales and pages of the unit's two 16-key slabs.
+// Ring slot beside the codes: scales and pages of the unit's two 16-key
+// slabs, and the barrier of all that arrives in the slot.
 struct alignas(16) SlotInfo {
   float scale[4];  // key, value of slab 0, of slab 1
   int page[2];     // -1: nothing to see
+  uint64_t full;
 };
 
 struct StreamArgs {
@@ -159,6 +162,17 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
                : "memory");
 }
 
+__device__ __forceinline__ void cp_async_wait_all() {
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// A load that stays where it is written, ahead of its use.
+__device__ __forceinline__ int load_early(const int32_t* p) {
+  int v;
+  asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+
 // Factor of a key scale in the exponent; a page of zeros has scale 0 and
 // scores 0, which any finite factor keeps.
 __device__ __forceinline__ float KeyFactor(float scale, float scale_log2) {
@@ -173,15 +187,6 @@ __device__ __forceinline__ float2 JoinFactors(float* top, float* sum, float2 ms)
   *sum = fmaf(ms.y, h, *sum * f);
   *top = grown;
   return make_float2(f, h);
-}
-
-__device__ __forceinline__ void JoinPart(float* top, float* sum, float4* v, float2 ms, float4 y) {
-  const float2 factors = JoinFactors(top, sum, ms);
-  const float f = factors.x, h = factors.y;
-  v->x = fmaf(y.x, h, v->x * f);
-  v->y = fmaf(y.y, h, v->y * f);
-  v->z = fmaf(y.z, h, v->z * f);
-  v->w = fmaf(y.w, h, v->w * f);
 }
 
 // One (sequence, kv head).  Its units have numbers begin, begin + 1, ...; the
@@ -218,9 +223,9 @@ struct ItemAt {
 };
 
 struct alignas(16) StreamShared {
-  int64_t sum[2][kStreamWarps];
-  ItemAt first[kStreamWarps];  // the item at each warp's first unit; seq -1: none
-  ItemAt part[2];              // items that this CTA shares with others
+  ItemAt group[kStreamWarps + 1];  // items to join: one begun before the CTA, then by warp
+  int rows[kStreamWarps + 1];      // their rows; 0: none
+  ItemAt part[2];                  // items that this CTA shares with others
   int has[2], last[2];
 };
 
@@ -239,30 +244,103 @@ constexpr size_t StreamSmem(int rows) {
          sizeof(StreamShared) + kStreamWarps * JoinFloats(rows) * sizeof(float);
 }
 
-// Sum of a value over the block and over the threads before this one; `slot`
-// is a row of sums that no other call uses.
-__device__ __forceinline__ int64_t BlockSum(int64_t mine, int64_t* slot, int64_t* before) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// n / d, in 32 bits where they hold it.
+__device__ __forceinline__ int64_t Divide(int64_t n, int64_t d) {
+  if (((n | d) >> 31) == 0) return static_cast<uint32_t>(n) / static_cast<uint32_t>(d);
+  return n / d;
+}
+
+// Sum of a value over the warp; `before`: over the lanes before this one.
+__device__ __forceinline__ int64_t WarpSum(int64_t mine, int64_t* before) {
   int64_t inclusive = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int64_t v = __shfl_up_sync(0xFFFFFFFFu, inclusive, o);
-    if (lane >= o) inclusive += v;
+    if ((threadIdx.x & 31) >= o) inclusive += v;
   }
-  if (lane == 31) slot[warp] = inclusive;
-  __syncthreads();
-  int64_t total = 0;
   *before = inclusive - mine;
-#pragma unroll
-  for (int w = 0; w < kStreamWarps; ++w) {
-    if (w < warp) *before += slot[w];
-    total += slot[w];
-  }
-  return total;
+  return __shfl_sync(0xFFFFFFFFu, inclusive, 31);
 }
 
+// How the units are numbered and shared out; every warp works it out for
+// itself, lane i from sequences [i * per, (i + 1) * per).
+struct Division {
+  ItemAt item;       // the lane's only sequence, where per is 1
+  int per;
+  int align;         // room of an item is a multiple of this
+  int64_t width;     // numbers of a warp
+  int64_t begin, end;  // of the lane's sequences
+
+  __device__ __forceinline__ explicit Division(const CacheAttnArgs& a) {
+    const int lane = threadIdx.x & 31, seqs = a.cache.num_seqs;
+    per = (seqs + 31) / 32;
+    const int first = min(seqs, lane * per), last = min(seqs, first + per);
+    int64_t mine = 0, before;
+    item.units = 0;
+    for (item.seq = first; item.seq < last; ++item.seq) {
+      item.Load(a, 1);
+      mine += item.units;
+    }
+    const int64_t units = WarpSum(mine, &before) * a.cache.kv_heads;
+    width = Divide(units + gridDim.x * kStreamWarps - 1, gridDim.x * kStreamWarps);
+    // CTAs that the items would take with a begin of their own.
+    const int wide = static_cast<int>(max(width, static_cast<int64_t>(kMinUnits))) * kStreamWarps;
+    int64_t ctas = 0, ctas_before;
+    if (per == 1) {
+      ctas = (item.units + wide - 1) / wide;
+    } else {
+      for (item.seq = first; item.seq < last; ++item.seq) {
+        item.Load(a, wide);
+        ctas += item.room / wide;
+      }
+    }
+    const int64_t all = WarpSum(ctas, &ctas_before) * a.cache.kv_heads;
+    align = 1;
+    if (all <= gridDim.x) {
+      align = wide;
+      width = wide / kStreamWarps;
+      mine = ctas * align;
+      before = ctas_before * align;
+    }
+    if (per == 1) {
+      item.seq = first;
+      item.room = static_cast<int>(mine);
+    }
+    begin = before * a.cache.kv_heads;
+    end = begin + mine * a.cache.kv_heads;
+  }
+
+  // The item at number p (the same in all lanes); seq -1 behind the last.
+  __device__ __forceinline__ ItemAt Find(const CacheAttnArgs& a, int64_t p) const {
+    ItemAt at;
+    at.seq = -1;
+    const uint32_t here = __ballot_sync(0xFFFFFFFFu, begin <= p && p < end);
+    if (here == 0) return at;
+    const int lane = __ffs(here) - 1;
+    at.begin = __shfl_sync(0xFFFFFFFFu, begin, lane);
+    if (per == 1) {
+      at.seq = __shfl_sync(0xFFFFFFFFu, item.seq, lane);
+      at.first = __shfl_sync(0xFFFFFFFFu, item.first, lane);
+      at.count = __shfl_sync(0xFFFFFFFFu, item.count, lane);
+      at.length = __shfl_sync(0xFFFFFFFFu, item.length, lane);
+      at.units = __shfl_sync(0xFFFFFFFFu, item.units, lane);
+      at.room = __shfl_sync(0xFFFFFFFFu, item.room, lane);
+    } else {
+      for (at.seq = lane * per;; ++at.seq) {
+        at.Load(a, align);
+        const int64_t heads = static_cast<int64_t>(at.room) * a.cache.kv_heads;
+        if (p < at.begin + heads) break;
+        at.begin += heads;
+      }
+    }
+    at.head = static_cast<int>(Divide(p - at.begin, at.room));
+    at.begin += static_cast<int64_t>(at.head) * at.room;
+    return at;
+  }
+};
+
 template <int kNT>
-__global__ void __launch_bounds__(kStreamThreads, 1)
+__global__ void __launch_bounds__(kStreamThreads + 128, 1)
     cache_attention_stream_kernel(const __grid_constant__ CUtensorMap map_k,
                                   const __grid_constant__ CUtensorMap map_v,
                                   const StreamArgs args) {
@@ -274,162 +352,140 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
                                              ~static_cast<uintptr_t>(1023));
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
-  uint8_t* ring = smem + warp * (kStages * 2 * kUnitTile);
+  // The rings of this warp, or (producers) of the one that this lane serves.
+  const bool producer = warp >= kStreamWarps;
+  const int mine_warp = producer ? (warp - kStreamWarps) * 2 + (lane & 1) : warp;
+  uint8_t* ring = smem + mine_warp * (kStages * 2 * kUnitTile);
   SlotInfo* info = reinterpret_cast<SlotInfo*>(smem + kStreamWarps * kStages * 2 * kUnitTile) +
-                   warp * kStages;
-  uint64_t* full = reinterpret_cast<uint64_t*>(
-                       smem + kStreamWarps * kStages * (2 * kUnitTile + sizeof(SlotInfo))) +
-                   warp * kStages;
+                   mine_warp * kStages;
+  uint64_t* empty = reinterpret_cast<uint64_t*>(
+                        smem + kStreamWarps * kStages * (2 * kUnitTile + sizeof(SlotInfo))) +
+                    mine_warp * kStages;
   StreamShared& shared = *reinterpret_cast<StreamShared*>(
       smem + kStreamWarps * kStages * (2 * kUnitTile + sizeof(SlotInfo) + sizeof(uint64_t)));
   float* join = reinterpret_cast<float*>(&shared + 1);  // [warp][JoinFloats(join_rows)]
   const size_t join_floats = JoinFloats(args.join_rows);
   const int stats = args.join_rows * kCacheHeadDim;  // of a part: maxima and sums
   pdl_trigger();
-  if (lane == 0) {
-    // Lanes 0 and 1 each arrive for their codes and for their scales.
-    for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 4);
+  if (producer && lane < 2) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&info[i].full, 2);  // for the codes and for the scales
+      mbar_init(&empty[i], 1);
+    }
     fence_mbar_init();
-    tma_prefetch_map(&map_k);
-    tma_prefetch_map(&map_v);
-    shared.first[warp].seq = -1;
-    if (warp == 0) shared.has[0] = shared.has[1] = 0;
+    if (warp == kStreamWarps) {
+      tma_prefetch_map(lane == 0 ? &map_k : &map_v);
+      shared.has[lane] = 0;
+    }
   }
   pdl_wait();
 
-  // This warp's numbers [p0, p1), of the CTA's from `base` on, and the item at p0.
+  // This warp's numbers [p0, p1), of the CTA's from `base` on, and the item
+  // at p0 (producers: those of the lane's warp).
+  ItemAt item;
   int align = 1;
-  int64_t width;  // numbers of a warp
-  int64_t base;
-  int own_units = 0;
+  int64_t width, base, p0, p1;
   if (args.counters == nullptr) {  // the CTA has an item to itself
-    ItemAt item;
     item.seq = static_cast<int>(blockIdx.x) / cache.kv_heads;
     item.head = static_cast<int>(blockIdx.x) % cache.kv_heads;
     item.begin = 0;
     item.Load(a, 1);
+    if (item.units == 0) return;  // uniform over the CTA
     width = (item.units + kStreamWarps - 1) / kStreamWarps;
     base = 0;
-    own_units = item.units;
-    if (item.units == 0) return;  // uniform over the CTA
-    __syncthreads();
-    if (tid < kStreamWarps && tid * width < item.units) shared.first[tid] = item;
-    __syncthreads();
+    // The CTA's numbers end with its item: the next one is another CTA's.
+    p0 = mine_warp * width;
+    p1 = min(p0 + width, static_cast<int64_t>(item.units));
+    if (p0 >= item.units) item.seq = -1;
   } else {
-    const int per = (cache.num_seqs + kStreamThreads - 1) / kStreamThreads;
-    const int first = min(cache.num_seqs, tid * per), last = min(cache.num_seqs, first + per);
-    ItemAt item;
-    int64_t mine = 0, before;
-    for (item.seq = first; item.seq < last; ++item.seq) {
-      item.Load(a, 1);
-      mine += item.units;
-    }
-    const int64_t units = BlockSum(mine, shared.sum[0], &before) * cache.kv_heads;
-    width = (units + gridDim.x * kStreamWarps - 1) / (gridDim.x * kStreamWarps);
-    // CTAs that the items would take with a begin of their own.
-    const int wide = static_cast<int>(max(width, static_cast<int64_t>(kMinUnits))) * kStreamWarps;
-    int64_t ctas = 0;
-    if (per == 1) {
-      if (first < last) ctas = (item.units + wide - 1) / wide;
-    } else {
-      for (item.seq = first; item.seq < last; ++item.seq) {
-        item.Load(a, wide);
-        ctas += item.room / wide;
-      }
-    }
-    int64_t ctas_before;
-    const int64_t all = BlockSum(ctas, shared.sum[1], &ctas_before) * cache.kv_heads;
-    if (all <= gridDim.x) {
-      align = wide;
-      width = wide / kStreamWarps;
-      mine = ctas * align;
-      before = ctas_before * align;
-    }
-    mine *= cache.kv_heads;
-    before *= cache.kv_heads;
+    const Division division(a);
+    align = division.align;
+    width = division.width;
     base = width * kStreamWarps * blockIdx.x;
-    if (base < before + mine && before < base + width * kStreamWarps) {
-      // Some warps of the CTA begin in this thread's sequences.
-      for (int s = first; s < last; ++s) {
-        item.seq = s;
-        if (per > 1) item.Load(a, align);
-        else item.room = (item.units + align - 1) / align * align;
-        const int64_t span = static_cast<int64_t>(item.room) * cache.kv_heads;
-        for (int w = 0; w < kStreamWarps; ++w) {
-          const int64_t p = base + w * width;
-          if (p < before || p >= before + span) continue;
-          item.head = static_cast<int>((p - before) / item.room);
-          item.begin = before + static_cast<int64_t>(item.head) * item.room;
-          shared.first[w] = item;
-        }
-        before += span;
-      }
+    p0 = base + mine_warp * width;
+    p1 = p0 + width;
+    item = division.Find(a, __shfl_sync(0xFFFFFFFFu, p0, 0));
+    if (producer) {
+      const ItemAt second = division.Find(a, __shfl_sync(0xFFFFFFFFu, p0, 1));
+      if (lane & 1) item = second;
     }
-    __syncthreads();
   }
-  // Without counters a CTA's numbers end with its item, else its last warps
-  // would go on to the next one, which is another CTA's.
-  const int64_t p0 = base + warp * width;
-  const int64_t p1 = args.counters == nullptr ? min(p0 + width, static_cast<int64_t>(own_units))
-                                              : p0 + width;
-  ItemAt item = shared.first[warp];
+  __syncthreads();  // the barriers are initialised
 
-  // The unit to load next, and the page of this lane's slab (lanes 0 and 1).
-  ItemAt fetch = item;
-  int64_t fetch_at = item.seq < 0 ? p1 : p0;
-  int fetch_page = -1;
-  bool fetch_slot = false;  // whether this lane's slab has tokens
-  auto look_up = [&] {
-    while (fetch_at < p1 && fetch_at >= fetch.end()) {
-      if (!fetch.Next(a, align)) {
-        fetch_at = p1;
+  // Registers: 384 threads start with 168 each.  The warpgroups that compute
+  // take 224 and leave the producer's 56.
+  if (producer) {
+    registers_shrink<56>();
+    // Lanes 0 and 1 fill a warp's ring each: the codes of a unit (one box, or two of 16
+    // keys), its scales and pages, the page numbers looked up one unit ahead.
+    const int box = min(kUnit, 1 << cache.page_shift);  // rows of a TMA box
+    int64_t at = lane < 2 && item.seq >= 0 ? p0 : p1;
+    int page[2] = {-1, -1}, tokens = 0, sent = 0;
+    auto look_up = [&] {
+      while (at < p1 && at >= item.end()) at = item.Next(a, align) ? item.begin : p1;
+      if (at >= p1) return;
+      const int token = static_cast<int>(at - item.begin) * kUnit;
+      tokens = item.length - token;
+      const int32_t* table = cache.table + static_cast<int64_t>(item.seq) * cache.max_pages;
+      if (tokens > 0) page[0] = load_early(table + (token >> cache.page_shift));
+      if (tokens > 16 && box < kUnit) page[1] = load_early(table + ((token + 16) >> cache.page_shift));
+    };
+    look_up();
+    uint64_t idle_since = 0;
+    while (__any_sync(0xFFFFFFFFu, at < p1)) {
+      const int stage = sent % kStages;
+      const bool ready = at < p1 && (sent < kStages ||
+                                     mbar_test_wait(&empty[stage], static_cast<uint32_t>(sent / kStages - 1) & 1u));
+      if (ready) {
+        int now[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {  // the pages of the unit's slabs
+          now[h] = tokens > h * 16 ? page[box < kUnit ? h : 0] : -1;
+          if (tokens > h * 16 && (now[h] < 0 || now[h] >= cache.pages)) {
+            atomicOr(a.err, kErrBadArgument);
+            now[h] = -1;
+          }
+          info[stage].page[h] = now[h];
+          if (now[h] >= 0) {
+            const int64_t scale = static_cast<int64_t>(now[h]) * cache.kv_heads + item.head;
+            cp_async_4(&info[stage].scale[2 * h], cache.key_scales + scale);
+            cp_async_4(&info[stage].scale[2 * h + 1], cache.value_scales + scale);
+          } else {
+            info[stage].scale[2 * h] = info[stage].scale[2 * h + 1] = 1.0f;
+          }
+        }
+        const int loads = (now[0] >= 0) + (box < kUnit && now[1] >= 0);
+        mbar_arrive_expect_tx(&info[stage].full, static_cast<uint32_t>(2 * loads * box * kCacheHeadDim));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (now[h] < 0 || (h == 1 && box == kUnit)) continue;
+          const int token = static_cast<int>(at - item.begin) * kUnit + h * 16;
+          const int row = ((now[h] * cache.kv_heads + item.head) << cache.page_shift) +
+                          (token & ((1 << cache.page_shift) - 1));
+          uint8_t* dst = ring + stage * 2 * kUnitTile + h * 16 * kCacheHeadDim;
+          tma_load_2d(dst, &map_k, &info[stage].full, 0, row);
+          tma_load_2d(dst + kUnitTile, &map_v, &info[stage].full, 0, row);
+        }
+        cp_async_arrive(&info[stage].full);
+        ++sent;
+        ++at;
+        look_up();
+      }
+      // Bounded: warps that give up waiting still free their slots, so this
+      // one ends too.
+      if (__any_sync(0xFFFFFFFFu, ready)) {
+        idle_since = 0;
+      } else if (idle_since == 0) {
+        idle_since = global_timer_ns();
+      } else if (global_timer_ns() - idle_since > 2 * kWaitLimitNs) {
+        if (lane == 0) atomicOr(a.err, kErrWaitTimeout);
         break;
       }
-      fetch_at = fetch.begin;
     }
-    if (fetch_at >= p1) return;
-    const int token = static_cast<int>(fetch_at - fetch.begin) * kUnit + (lane & 1) * 16;
-    fetch_slot = lane < 2 && token < fetch.length;
-    if (fetch_slot)
-      fetch_page = cache.table[static_cast<int64_t>(fetch.seq) * cache.max_pages +
-                               (token >> cache.page_shift)];
-  };
-  const int box = min(kUnit, 1 << cache.page_shift);  // rows of a TMA box
-  auto issue = [&](int stage) {
-    if (fetch_at >= p1) return;
-    if (lane < 2) {
-      uint64_t* bar = &full[stage];
-      int page = fetch_slot ? fetch_page : -1;
-      if (fetch_slot && (page < 0 || page >= cache.pages)) {
-        atomicOr(a.err, kErrBadArgument);
-        page = -1;
-      }
-      info[stage].page[lane] = page;
-      if (page >= 0) {
-        const int64_t at = static_cast<int64_t>(page) * cache.kv_heads + fetch.head;
-        cp_async_4(&info[stage].scale[2 * lane], cache.key_scales + at);
-        cp_async_4(&info[stage].scale[2 * lane + 1], cache.value_scales + at);
-      } else {
-        info[stage].scale[2 * lane] = info[stage].scale[2 * lane + 1] = 1.0f;
-      }
-      if (page >= 0 && (lane == 0 || box < kUnit)) {
-        const int token = static_cast<int>(fetch_at - fetch.begin) * kUnit + lane * 16;
-        const int row = ((page * cache.kv_heads + fetch.head) << cache.page_shift) +
-                        (token & ((1 << cache.page_shift) - 1));
-        uint8_t* dst = ring + stage * 2 * kUnitTile + lane * 16 * kCacheHeadDim;
-        mbar_arrive_expect_tx(bar, 2 * box * kCacheHeadDim);
-        tma_load_2d(dst, &map_k, bar, 0, row);
-        tma_load_2d(dst + kUnitTile, &map_v, bar, 0, row);
-      } else {
-        mbar_arrive(bar);
-      }
-      cp_async_arrive(bar);
-    }
-    ++fetch_at;
-    look_up();
-  };
-  look_up();
-  for (int i = 0; i < kStages; ++i) issue(i);
+    cp_async_wait_all();
+    return;
+  }
+  registers_grow<224>();
 
   // kappa(g) and kappa(2c), see above.
   const int key_g = ((g & 1) << 2) | (g & 2) | (g >> 2);
@@ -451,6 +507,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
            (it.head * a.group.d + r - token * a.group.d) * kCacheHeadDim;
   };
 
+  const ItemAt started = item;
   int64_t at = p0;
   int done = 0;  // units of this warp so far
   bool ok = true;  // once a wait ran out, no other is begun
@@ -500,7 +557,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
       }
       for (; at < end; ++at) {
         const int stage = done % kStages;
-        ok = ok && mbar_wait(&full[stage], static_cast<uint32_t>(done / kStages) & 1u, a.err);
+        ok = ok && mbar_wait(&info[stage].full, static_cast<uint32_t>(done / kStages) & 1u, a.err);
         __syncwarp();
         const uint8_t* keys = ring + stage * 2 * kUnitTile;
         const uint8_t* values = keys + kUnitTile;
@@ -617,7 +674,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
         }
         ++done;
         __syncwarp();
-        issue(stage);
+        if (lane == 0) mbar_arrive(&empty[stage]);
       }
 
       // Out, or a part: of an item begun before p0 in `join`, of one that goes
@@ -658,31 +715,64 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     at = min(p1, item.begin + item.room);
     if (at >= p1 || !item.Next(a, align)) break;
   }
-  __syncthreads();
+  if (lane == 0) {
+    shared.group[warp + 1] = item;
+    shared.rows[warp + 1] = tail ? item.count * a.group.d : 0;
+    if (warp == 0) {
+      const bool begun_before = started.seq >= 0 && started.begin < base && base < started.end();
+      shared.group[0] = started;
+      shared.rows[0] = begun_before ? started.count * a.group.d : 0;
+    }
+  }
+  named_barrier(1, kStreamThreads);
 
-  // Joins: an item is the work of the warp that begins it (warp 0 also has
-  // the one begun before the CTA).
+  // Joins: rows of the items that span warps, dealt out over the warps.
   const int64_t cta_end = base + width * kStreamWarps;
   auto store_vector = [&](const ItemAt& it, int r, int d, float4 v, float sum) {
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     *reinterpret_cast<uint2*>(out_row(it, r) + d) =
         make_uint2(pack_half2(v.x * inv, v.y * inv), pack_half2(v.z * inv, v.w * inv));
   };
-  auto join_warps = [&](const ItemAt& it, bool begun) {
-    const int last = static_cast<int>(min(static_cast<int64_t>(kStreamWarps),
-                                          (it.end() - 1 - base) / width + 1));
-    const int slot = begun ? 1 : 0;
+  int task = warp;  // this warp's next row among all groups' rows
+#pragma unroll 1
+  for (int i = 0, before = 0; i <= kStreamWarps; ++i) {
+    const int rows = shared.rows[i];
+    if (task >= before + rows) {
+      before += rows;
+      continue;
+    }
+    // Group 0 is the item begun before the CTA, group w + 1 the one begun by
+    // warp w: that part lies in the warp's ring, the others' in `join`.
+    const ItemAt it = shared.group[i];
+    const bool begun = i > 0;
+    const int from = begun ? i - 1 : 0;
+    const int to = static_cast<int>(min(static_cast<int64_t>(kStreamWarps),
+                                        Divide(it.end() - 1 - base, width) + 1));
+    auto part_of = [&](int w) {
+      return begun && w == from ? reinterpret_cast<const float*>(smem + w * (kStages * 2 * kUnitTile))
+                                : join + w * join_floats;
+    };
     const bool whole = begun && it.end() <= cta_end;
-    float* dst = whole ? nullptr : args.parts + (static_cast<int64_t>(blockIdx.x) * 2 + slot) * join_floats;
-    const int d = lane * 4;
-    for (int r = 0; r < it.count * a.group.d; ++r) {
-      float top = -INFINITY, sum = 0.0f;
+    float* dst = whole ? nullptr : args.parts + (static_cast<int64_t>(blockIdx.x) * 2 + begun) * join_floats;
+    for (; task < before + rows; task += kStreamWarps) {
+      const int r = task - before, d = lane * 4;
+      // Lane w looks after the statistics of warp w's part.
+      float2 ms = make_float2(-INFINITY, 0.0f);
+      if (lane >= from && lane < to)
+        ms = *reinterpret_cast<const float2*>(part_of(lane) + stats + 2 * r);
+      const float top = warp_max(ms.x);
+      const float f = ex2_approx(ms.x - (top == -INFINITY ? 0.0f : top));
+      const float sum = warp_sum(ms.y * f);
       float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-      for (int w = warp; w < last; ++w) {
-        const float* p = w == warp && begun ? reinterpret_cast<const float*>(ring) : join + w * join_floats;
-        JoinPart(&top, &sum, &v, *reinterpret_cast<const float2*>(p + stats + 2 * r),
-                 *reinterpret_cast<const float4*>(p + r * kCacheHeadDim + d));
+#pragma unroll
+      for (int w = 0; w < kStreamWarps; ++w) {
+        const float fw = __shfl_sync(0xFFFFFFFFu, f, w);
+        if (w < from || w >= to) continue;
+        const float4 y = *reinterpret_cast<const float4*>(part_of(w) + r * kCacheHeadDim + d);
+        v.x = fmaf(y.x, fw, v.x);
+        v.y = fmaf(y.y, fw, v.y);
+        v.z = fmaf(y.z, fw, v.z);
+        v.w = fmaf(y.w, fw, v.w);
       }
       if (whole) {
         store_vector(it, r, d, v, sum);
@@ -691,47 +781,53 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
         if (lane == 0) *reinterpret_cast<float2*>(dst + stats + 2 * r) = make_float2(top, sum);
       }
     }
+    before += rows;
     if (!whole && lane == 0) {
-      shared.part[slot] = it;
-      shared.has[slot] = 1;
+      shared.part[begun] = it;
+      shared.has[begun] = 1;
     }
-  };
-  if (warp == 0) {
-    const ItemAt it = shared.first[0];
-    if (it.seq >= 0 && it.begin < base && base < it.end()) join_warps(it, false);
   }
-  if (tail) join_warps(item, true);
-  __syncthreads();
+  named_barrier(1, kStreamThreads);
 
   // The last CTA of an item to arrive joins its parts, in CTA order.
   if (shared.has[0] + shared.has[1] == 0) return;
   const int64_t cta_width = width * kStreamWarps;
   if (tid < 2 && shared.has[tid] != 0) {
     const ItemAt it = shared.part[tid];
-    const int64_t parts = (it.end() - 1) / cta_width - it.begin / cta_width;
+    const int64_t parts = Divide(it.end() - 1, cta_width) - Divide(it.begin, cta_width);
     uint32_t* counter = args.counters + static_cast<int64_t>(it.seq) * cache.kv_heads + it.head;
-    __threadfence();
-    const bool last = atomicAdd(counter, 1u) == static_cast<uint32_t>(parts);
+    const bool last = atom_add_acq_rel(counter, 1u) == static_cast<uint32_t>(parts);
     if (last) *counter = 0;
-    __threadfence();
     shared.last[tid] = last;
   }
-  __syncthreads();
+  named_barrier(1, kStreamThreads);
   for (int slot = 0; slot < 2; ++slot) {
     if (shared.has[slot] == 0 || shared.last[slot] == 0) continue;
     const ItemAt it = shared.part[slot];
-    const int first = static_cast<int>(it.begin / cta_width);
-    const int last = static_cast<int>((it.end() - 1) / cta_width);
+    const int first = static_cast<int>(Divide(it.begin, cta_width));
+    const int last = static_cast<int>(Divide(it.end() - 1, cta_width));
     for (int i = tid; i < it.count * a.group.d * (kCacheHeadDim / 4); i += kStreamThreads) {
       const int r = i / (kCacheHeadDim / 4), d = i % (kCacheHeadDim / 4) * 4;
-      float top = -INFINITY, sum = 0.0f;
+      // The first CTA began the item: its part is its second, the others' their first.
+      auto part_of = [&](int x) {
+        return args.parts + (static_cast<int64_t>(x) * 2 + (x == first ? 1 : 0)) * join_floats;
+      };
+      float top = -INFINITY;
+#pragma unroll 8
+      for (int x = first; x <= last; ++x) top = fmaxf(top, __ldcg(part_of(x) + stats + 2 * r));
+      const float zero = top == -INFINITY ? 0.0f : top;
+      float sum = 0.0f;
       float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 8
       for (int x = first; x <= last; ++x) {
-        // The first CTA began the item: its part is its second, the others' their first.
-        const float* p = args.parts + (static_cast<int64_t>(x) * 2 + (x == first ? 1 : 0)) * join_floats;
-        const float2 ms = __ldcg(reinterpret_cast<const float2*>(p + stats + 2 * r));
-        JoinPart(&top, &sum, &v, ms, __ldcg(reinterpret_cast<const float4*>(p + r * kCacheHeadDim + d)));
+        const float2 ms = __ldcg(reinterpret_cast<const float2*>(part_of(x) + stats + 2 * r));
+        const float4 y = __ldcg(reinterpret_cast<const float4*>(part_of(x) + r * kCacheHeadDim + d));
+        const float f = ex2_approx(ms.x - zero);
+        v.x = fmaf(y.x, f, v.x);
+        v.y = fmaf(y.y, f, v.y);
+        v.z = fmaf(y.z, f, v.z);
+        v.w = fmaf(y.w, f, v.w);
+        sum = fmaf(ms.y, f, sum);
       }
       store_vector(it, r, d, v, sum);
     }
@@ -1319,17 +1415,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     if (at < here && (pair || g == 0))
       *reinterpret_cast<float2*>(part + stats_at + 2 * at) = make_float2(m, l);
     // The last part to arrive joins all of them, in split order.
-    __threadfence();
     named_barrier(1, 256);
     uint32_t* counter = args.counters + item;
     if (tid == 0) {
-      __threadfence();
-      s.last = atomicAdd(counter, 1u) == static_cast<uint32_t>(parts - 1);
+      s.last = atom_add_acq_rel(counter, 1u) == static_cast<uint32_t>(parts - 1);
       if (s.last) *counter = 0;
     }
     named_barrier(1, 256);
     if (!s.last) return;
-    __threadfence();
     const float* base_part = args.parts + item * args.splits * TilePartFloats(args.tile_rows);
     for (int i = tid; i < 8 * args.tile_rows; i += 256) {
       const int row = i & (args.tile_rows - 1), d16 = i / args.tile_rows;  // 16 columns of a row
@@ -1418,7 +1511,7 @@ void LaunchStream(const StreamArgs& args, unsigned ctas, const CUtensorMap& map_
                   const CUtensorMap& map_v, cudaStream_t stream) {
   SetMaxDynamicSmem(reinterpret_cast<const void*>(cache_attention_stream_kernel<kNT>),
                     static_cast<int>(StreamSmem<kNT>(8 * kNT)));
-  Launch(cache_attention_stream_kernel<kNT>, dim3(ctas), dim3(kStreamThreads),
+  Launch(cache_attention_stream_kernel<kNT>, dim3(ctas), dim3(kStreamThreads + 128),
          StreamSmem<kNT>(args.join_rows), stream, "cache attention kernel launch", map_k, map_v,
          args);
 }
