@@ -746,8 +746,9 @@ __global__ void __launch_bounds__(kStreamThreads + 128, 1)
     const ItemAt it = shared.group[i];
     const bool begun = i > 0;
     const int from = begun ? i - 1 : 0;
-    const int to = static_cast<int>(min(static_cast<int64_t>(kStreamWarps),
-                                        Divide(it.end() - 1 - base, width) + 1));
+    // Bit w: warp w has a part.
+    const uint32_t members = __ballot_sync(
+        0xFFFFFFFFu, lane >= from && lane < kStreamWarps && base + lane * width < it.end());
     auto part_of = [&](int w) {
       return begun && w == from ? reinterpret_cast<const float*>(smem + w * (kStages * 2 * kUnitTile))
                                 : join + w * join_floats;
@@ -758,7 +759,7 @@ __global__ void __launch_bounds__(kStreamThreads + 128, 1)
       const int r = task - before, d = lane * 4;
       // Lane w looks after the statistics of warp w's part.
       float2 ms = make_float2(-INFINITY, 0.0f);
-      if (lane >= from && lane < to)
+      if (members >> lane & 1u)
         ms = *reinterpret_cast<const float2*>(part_of(lane) + stats + 2 * r);
       const float top = warp_max(ms.x);
       const float f = ex2_approx(ms.x - (top == -INFINITY ? 0.0f : top));
@@ -767,7 +768,7 @@ __global__ void __launch_bounds__(kStreamThreads + 128, 1)
 #pragma unroll
       for (int w = 0; w < kStreamWarps; ++w) {
         const float fw = __shfl_sync(0xFFFFFFFFu, f, w);
-        if (w < from || w >= to) continue;
+        if ((members >> w & 1u) == 0) continue;
         const float4 y = *reinterpret_cast<const float4*>(part_of(w) + r * kCacheHeadDim + d);
         v.x = fmaf(y.x, fw, v.x);
         v.y = fmaf(y.y, fw, v.y);
@@ -812,22 +813,35 @@ __global__ void __launch_bounds__(kStreamThreads + 128, 1)
       auto part_of = [&](int x) {
         return args.parts + (static_cast<int64_t>(x) * 2 + (x == first ? 1 : 0)) * join_floats;
       };
-      float top = -INFINITY;
-#pragma unroll 8
-      for (int x = first; x <= last; ++x) top = fmaxf(top, __ldcg(part_of(x) + stats + 2 * r));
-      const float zero = top == -INFINITY ? 0.0f : top;
-      float sum = 0.0f;
+      float top = -INFINITY, sum = 0.0f;
       float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-      for (int x = first; x <= last; ++x) {
-        const float2 ms = __ldcg(reinterpret_cast<const float2*>(part_of(x) + stats + 2 * r));
-        const float4 y = __ldcg(reinterpret_cast<const float4*>(part_of(x) + r * kCacheHeadDim + d));
-        const float f = ex2_approx(ms.x - zero);
-        v.x = fmaf(y.x, f, v.x);
-        v.y = fmaf(y.y, f, v.y);
-        v.z = fmaf(y.z, f, v.z);
-        v.w = fmaf(y.w, f, v.w);
-        sum = fmaf(ms.y, f, sum);
+      for (int x0 = first; x0 <= last; x0 += 8) {  // eight parts' loads in flight
+        float2 ms[8];
+        float4 y[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          ms[x] = make_float2(-INFINITY, 0.0f);
+          y[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (x0 + x > last) continue;
+          ms[x] = __ldcg(reinterpret_cast<const float2*>(part_of(x0 + x) + stats + 2 * r));
+          y[x] = __ldcg(reinterpret_cast<const float4*>(part_of(x0 + x) + r * kCacheHeadDim + d));
+        }
+        float grown = top;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) grown = fmaxf(grown, ms[x].x);
+        const float zero = grown == -INFINITY ? 0.0f : grown;
+        const float old = ex2_approx(top - zero);
+        top = grown;
+        v.x *= old, v.y *= old, v.z *= old, v.w *= old, sum *= old;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const float f = ex2_approx(ms[x].x - zero);
+          v.x = fmaf(y[x].x, f, v.x);
+          v.y = fmaf(y[x].y, f, v.y);
+          v.z = fmaf(y[x].z, f, v.z);
+          v.w = fmaf(y[x].w, f, v.w);
+          sum = fmaf(ms[x].y, f, sum);
+        }
       }
       store_vector(it, r, d, v, sum);
     }
