@@ -283,24 +283,26 @@ struct Division {
     }
     const int64_t units = WarpSum(mine, &before) * a.cache.kv_heads;
     width = Divide(units + gridDim.x * kStreamWarps - 1, gridDim.x * kStreamWarps);
-    // CTAs that the items would take with a begin of their own.
-    const int wide = static_cast<int>(max(width, static_cast<int64_t>(kMinUnits))) * kStreamWarps;
-    int64_t ctas = 0, ctas_before;
-    if (per == 1) {
-      ctas = (item.units + wide - 1) / wide;
-    } else {
-      for (item.seq = first; item.seq < last; ++item.seq) {
-        item.Load(a, wide);
-        ctas += item.room / wide;
-      }
-    }
-    const int64_t all = WarpSum(ctas, &ctas_before) * a.cache.kv_heads;
     align = 1;
-    if (all <= gridDim.x) {
-      align = wide;
-      width = wide / kStreamWarps;
-      mine = ctas * align;
-      before = ctas_before * align;
+    // Items with a begin of their own at a CTA, if they all fit.
+    if (seqs * a.cache.kv_heads <= static_cast<int>(gridDim.x)) {
+      const int wide = static_cast<int>(max(width, static_cast<int64_t>(kMinUnits))) * kStreamWarps;
+      int64_t ctas = 0, ctas_before;
+      if (per == 1) {
+        ctas = (item.units + wide - 1) / wide;
+      } else {
+        for (item.seq = first; item.seq < last; ++item.seq) {
+          item.Load(a, wide);
+          ctas += item.room / wide;
+        }
+      }
+      const int64_t all = WarpSum(ctas, &ctas_before) * a.cache.kv_heads;
+      if (all <= gridDim.x) {
+        align = wide;
+        width = wide / kStreamWarps;
+        mine = ctas * align;
+        before = ctas_before * align;
+      }
     }
     if (per == 1) {
       item.seq = first;
