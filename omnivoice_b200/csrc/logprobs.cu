@@ -27,6 +27,7 @@ namespace {
 
 constexpr int kMaxTopK = 32;
 constexpr float kLog2E = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 
 struct LogprobArgs {
   const void* logits;
@@ -126,6 +127,12 @@ __device__ __forceinline__ void StoreNothing(const LogprobArgs& a, int64_t out, 
   }
 }
 
+// n / d, in 32 bits where they hold it.
+__device__ __forceinline__ int64_t Quotient(int64_t n, int d) {
+  if (n >> 31 == 0) return static_cast<uint32_t>(n) / static_cast<uint32_t>(d);
+  return n / d;
+}
+
 // The item's target, or -1.
 __device__ __forceinline__ int Target(const LogprobArgs& a, int64_t out, bool report) {
   const int t = a.targets[out];
@@ -134,132 +141,9 @@ __device__ __forceinline__ int Target(const LogprobArgs& a, int64_t out, bool re
   return -1;
 }
 
-// ------------------------------------------- short rows: one warp per item
+// ------------------------------------------------- exponents by logits type
 
-constexpr int kWarps = 8;
-constexpr int kWarpKeys = 64;
-
-// The whole group sits in registers, value j in lane j % 32.
-template <typename T, int kPer>
-__global__ void __launch_bounds__(kWarps * 32) logprobs_warp_kernel(const LogprobArgs a) {
-  __shared__ uint64_t s_keys[kWarps][kWarpKeys];
-  pdl_trigger();
-  pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  if (item >= a.rows * a.codebooks) return;
-  const int64_t row = item / a.codebooks;
-  const int codebook = static_cast<int>(item % a.codebooks);
-  const int64_t out = codebook * a.rows + row;
-  const T* src = static_cast<const T*>(a.logits) + row * a.ld + static_cast<int64_t>(codebook) * a.vocab;
-  float x[kPer];
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int j = lane + 32 * i;
-    x[i] = j < a.vocab ? ToFloat(src[j]) : -INFINITY;
-  }
-  const int target = Target(a, out, lane == 0);
-  const float xt = target >= 0 ? ToFloat(src[target]) : 0.0f;
-  float top = x[0];
-#pragma unroll
-  for (int i = 1; i < kPer; ++i) top = MaxNan(top, x[i]);
-  float m = top;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = MaxNan(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-  if (!(fabsf(m) < INFINITY)) {
-    StoreNothing(a, out, lane);
-    return;
-  }
-  float z = 0.0f, w = 0.0f;
-  int ahead = 0;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const float d = fmaxf(x[i] - m, -1e30f);  // finite, so that 0 * d is 0 for a closed token
-    const float e = Exp2Approx(d * kLog2E);
-    z += e;
-    w = fmaf(e, d, w);
-  }
-  if (a.rank != nullptr) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int j = lane + 32 * i;
-      ahead += (x[i] > xt || (x[i] == xt && j < target)) ? 1 : 0;
-    }
-    ahead = __reduce_add_sync(0xFFFFFFFFu, ahead);
-  }
-  z = warp_sum(z);
-  w = warp_sum(w);
-  const float log_z = logf(z);
-  if (lane == 0) {
-    a.logprob[out] = target >= 0 ? (xt - m) - log_z : 0.0f;
-    if (a.entropy != nullptr) a.entropy[out] = log_z - w / z;
-    if (a.rank != nullptr) a.rank[out] = target >= 0 ? ahead : -1;
-  }
-  const int k = a.top_k;
-  if (k == 0) return;
-  int32_t* ids = a.top_ids + out * k;
-  float* logprobs = a.top_logprobs + out * k;
-  // k lanes hold a value of at least the k-th greatest lane maximum.
-  const float threshold = WarpKth(top, k);
-  uint64_t* keys = s_keys[threadIdx.x >> 5];
-  int n = 0;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const bool pass = x[i] >= threshold && lane + 32 * i < a.vocab;
-    const uint32_t mask = __ballot_sync(0xFFFFFFFFu, pass);
-    if (mask == 0) continue;
-    const int at = n + __popc(mask & ((1u << lane) - 1u));
-    if (pass && at < kWarpKeys) keys[at] = AlternativeKey(x[i], lane + 32 * i);
-    n += __popc(mask);
-  }
-  __syncwarp();
-  if (n <= kWarpKeys) {
-    const uint64_t k0 = lane < n ? keys[lane] : 0, k1 = lane + 32 < n ? keys[lane + 32] : 0;
-    int r0 = 0, r1 = 0;
-    for (int j = 0; j < n; ++j) {
-      const uint64_t other = keys[j];
-      r0 += other > k0 ? 1 : 0;
-      r1 += other > k1 ? 1 : 0;
-    }
-    if (k0 != 0 && r0 < k) {
-      ids[r0] = KeyIndex(k0);
-      logprobs[r0] = (KeyValue(k0) - m) - log_z;
-    }
-    if (k1 != 0 && r1 < k) {
-      ids[r1] = KeyIndex(k1);
-      logprobs[r1] = (KeyValue(k1) - m) - log_z;
-    }
-    return;
-  }
-  // Many equal or closed values: one alternative after the other.
-  uint64_t last = ~uint64_t{0};
-  for (int r = 0; r < k; ++r) {
-    uint64_t best = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int j = lane + 32 * i;
-      const uint64_t key = j < a.vocab ? AlternativeKey(x[i], j) : 0;
-      if (key < last && key > best) best = key;
-    }
-    last = WarpMaxKey(best);
-    if (lane == 0) {
-      ids[r] = KeyIndex(last);
-      logprobs[r] = (KeyValue(last) - m) - log_z;
-    }
-  }
-}
-
-// ------------------------------ long rows: one CTA, or a cluster, per item
-
-constexpr int kThreads = 256;
-constexpr int kKeys = 1024;      // room for passing values between prunings
 constexpr int kVectors = 4;      // 16-byte vectors of a thread and chunk (Row::Top takes four)
-
-// Running maximum, Z = sum 2^t and W = sum 2^t t of what was read, with
-// t = Row<T>::Exponent(x, m).
-struct RowStats {
-  float m, z, w;
-};
 
 // 16 bytes of logits, and how their exponent t = (x - m) log2(e) is formed.
 // For float32 the difference comes first: a mask of the type's lowest value
@@ -331,7 +215,7 @@ struct Row<__half> {
     return fmaf(x, kLog2E, -scaled);
   }
   static __device__ __forceinline__ float LogProb(float x, float m, float log_z) {
-    return fmaf(Exponent(x, Scaled(m)), 0.6931471805599453f, -log_z);
+    return fmaf(Exponent(x, Scaled(m)), kLn2, -log_z);
   }
   static __device__ __forceinline__ float At(const uint4& q, int i) {
     const uint32_t w = i < 2 ? q.x : i < 4 ? q.y : i < 6 ? q.z : q.w;
@@ -376,6 +260,165 @@ struct Row<__half> {
     return __half2float(__ushort_as_half(static_cast<uint16_t>(
         x > 0.0f ? h - 1 : x == 0.0f ? 0x8001 : h + 1)));
   }
+};
+
+// ------------------------------------------- short rows: one warp per item
+
+constexpr int kWarps = 8;
+constexpr int kWarpKeys = 64;
+
+// The whole group sits in registers, value j in lane j % 32: a load, a
+// maximum, an exponential, two comparisons and a handful of sums for a value.
+// What bounds it is the instructions (about 20 for a value, with what a row
+// costs once), with the loads' latency hidden by the SM's 32 warps.
+template <typename T, int kPer>
+__global__ void __launch_bounds__(kWarps * 32, kPer <= 33 ? 4 : 2)
+    logprobs_warp_kernel(const LogprobArgs a) {
+  using R = Row<T>;
+  constexpr int kMasks = (kPer + 31) / 32;
+  __shared__ uint64_t s_keys[kWarps][kWarpKeys];
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+  if (item >= a.rows * a.codebooks) return;
+  const int64_t row = Quotient(item, a.codebooks);
+  const int codebook = static_cast<int>(item - row * a.codebooks);
+  const int64_t out = codebook * a.rows + row;
+  const T* src = static_cast<const T*>(a.logits) + row * a.ld + static_cast<int64_t>(codebook) * a.vocab;
+  float x[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int j = lane + 32 * i;
+    x[i] = j < a.vocab ? ToFloat(src[j]) : -INFINITY;
+  }
+  const int target = Target(a, out, lane == 0);
+  const float xt = target >= 0 ? ToFloat(src[target]) : INFINITY;
+  float top = x[0];
+#pragma unroll
+  for (int i = 1; i < kPer; ++i) top = MaxNan(top, x[i]);
+  float m = top;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = MaxNan(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  if (!(fabsf(m) < INFINITY)) {
+    StoreNothing(a, out, lane);
+    return;
+  }
+  const float scaled = R::Scaled(m);
+  float z = 0.0f, w = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    // Finite, so that 0 * t is 0 for a closed token.
+    const float t = fmaxf(R::Exponent(x[i], scaled), -16384.0f);
+    const float e = Exp2Approx(t);
+    z += e;
+    w = fmaf(e, t, w);
+  }
+  z = warp_sum(z);
+  w = warp_sum(w);
+  const float log_z = logf(z);
+  int ahead = 0;
+  if (a.rank != nullptr && target >= 0) {
+    bool equal = false;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      ahead += x[i] > xt ? 1 : 0;
+      equal |= x[i] == xt;
+    }
+    // More lanes than the target's hold its value, or that one may hold it
+    // twice: those with a lower index are ahead as well.
+    if (__popc(__ballot_sync(0xFFFFFFFFu, equal)) > 1 || xt == -INFINITY) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) ahead += x[i] == xt && lane + 32 * i < target ? 1 : 0;
+    } else if (equal) {
+      for (int j = lane; j < target; j += 32) ahead += ToFloat(src[j]) == xt ? 1 : 0;
+    }
+    ahead = __reduce_add_sync(0xFFFFFFFFu, ahead);
+  }
+  if (lane == 0) {
+    a.logprob[out] = target >= 0 ? R::LogProb(xt, m, log_z) : 0.0f;
+    if (a.entropy != nullptr) a.entropy[out] = fmaf(w / z, -kLn2, log_z);
+    if (a.rank != nullptr) a.rank[out] = target >= 0 ? ahead : -1;
+  }
+  const int k = a.top_k;
+  if (k == 0) return;
+  int32_t* ids = a.top_ids + out * k;
+  float* logprobs = a.top_logprobs + out * k;
+  // k lanes hold a value of at least the k-th greatest lane maximum.  Taking
+  // maxima one after the other is shorter than a sort up to about eight.
+  const float threshold = k <= 8 ? WarpKthOfFew(top, k) : WarpKth(top, k);
+  uint32_t masks[kMasks] = {};  // bit i % 32 of masks[i / 32]: x[i] passes
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    if (x[i] >= threshold) masks[i / 32] |= 1u << (i % 32);
+  int mine = 0;
+#pragma unroll
+  for (int i = 0; i < kMasks; ++i) {
+    // Values behind the group pass only where -inf does.
+    const int valid = (a.vocab - lane + 31) / 32 - 32 * i;
+    masks[i] &= valid >= 32 ? ~0u : valid <= 0 ? 0u : (1u << valid) - 1u;
+    mine += __popc(masks[i]);
+  }
+  int at = mine;  // inclusive, then exclusive count of the lanes before
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int before = __shfl_up_sync(0xFFFFFFFFu, at, o);
+    if (lane >= o) at += before;
+  }
+  const int n = __shfl_sync(0xFFFFFFFFu, at, 31);
+  at -= mine;
+  if (n <= kWarpKeys) {
+    uint64_t* keys = s_keys[threadIdx.x >> 5];
+#pragma unroll
+    for (int i = 0; i < kMasks; ++i) {
+      uint32_t mask = masks[i];
+      while (mask != 0) {
+        const int j = lane + 32 * (32 * i + __ffs(mask) - 1);
+        mask &= mask - 1;
+        keys[at++] = AlternativeKey(ToFloat(src[j]), j);
+      }
+    }
+    __syncwarp();
+    const uint64_t k0 = lane < n ? keys[lane] : 0, k1 = lane + 32 < n ? keys[lane + 32] : 0;
+    int r0 = 0, r1 = 0;
+    for (int j = 0; j < n; ++j) r0 += keys[j] > k0 ? 1 : 0;
+    if (n > 32)
+      for (int j = 0; j < n; ++j) r1 += keys[j] > k1 ? 1 : 0;
+    if (k0 != 0 && r0 < k) {
+      ids[r0] = KeyIndex(k0);
+      logprobs[r0] = R::LogProb(KeyValue(k0), m, log_z);
+    }
+    if (k1 != 0 && r1 < k) {
+      ids[r1] = KeyIndex(k1);
+      logprobs[r1] = R::LogProb(KeyValue(k1), m, log_z);
+    }
+    return;
+  }
+  // Many equal or closed values: one alternative after the other.
+  uint64_t last = ~uint64_t{0};
+  for (int r = 0; r < k; ++r) {
+    uint64_t best = 0;
+    for (int j = lane; j < a.vocab; j += 32) {
+      const uint64_t key = AlternativeKey(ToFloat(src[j]), j);
+      if (key < last && key > best) best = key;
+    }
+    last = WarpMaxKey(best);
+    if (lane == 0) {
+      ids[r] = KeyIndex(last);
+      logprobs[r] = R::LogProb(KeyValue(last), m, log_z);
+    }
+  }
+}
+
+// ------------------------------ long rows: one CTA, or a cluster, per item
+
+constexpr int kThreads = 256;
+constexpr int kKeys = 1024;      // room for passing values between prunings
+
+// Running maximum, Z = sum 2^t and W = sum 2^t t of what was read, with
+// t = Row<T>::Exponent(x, m).
+struct RowStats {
+  float m, z, w;
 };
 
 // To a maximum m >= s.m.
@@ -461,8 +504,8 @@ __global__ void __launch_bounds__(kThreads, 4)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int part = static_cast<int>(blockIdx.x % static_cast<unsigned>(cluster));
   const int64_t item = blockIdx.x / static_cast<unsigned>(cluster);
-  const int64_t row = item / a.codebooks;
-  const int codebook = static_cast<int>(item % a.codebooks);
+  const int64_t row = Quotient(item, a.codebooks);
+  const int codebook = static_cast<int>(item - row * a.codebooks);
   const int64_t out = codebook * a.rows + row;
   const T* src = static_cast<const T*>(a.logits) + row * a.ld + static_cast<int64_t>(codebook) * a.vocab;
   const int k = a.top_k;
@@ -737,7 +780,7 @@ __global__ void __launch_bounds__(kThreads, 4)
   if (tid == 0) {
     a.logprob[out] = target >= 0 ? R::LogProb(xt, total.m, log_z) : 0.0f;
     if (a.entropy != nullptr)
-      a.entropy[out] = fmaf(total.w / total.z, -0.6931471805599453f, log_z);
+      a.entropy[out] = fmaf(total.w / total.z, -kLn2, log_z);
     if (a.rank != nullptr) a.rank[out] = target >= 0 ? s.total_ahead : -1;
   }
   const int n = min(s.count, k);
