@@ -8,6 +8,7 @@
 // are rounded to 8 bits, which is the operator; everything before that is
 // float32.  Both kernels move bytes and nothing else: a written element costs
 // 2 bytes read and 1 written, a read one 1 and 2.
+#include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -210,10 +211,36 @@ void RequireAligned(const void* pointer, size_t align, const char* name) {
                                     "-byte aligned");
 }
 
+namespace {
+
+// The driver's single-attribute query: a third of the runtime's cost, and
+// each call asks it for about ten tensors.
+using PointerAttributeFn = CUresult (*)(void*, CUpointer_attribute, CUdeviceptr);
+PointerAttributeFn GetPointerAttribute() {
+  static PointerAttributeFn fn = [] {
+    void* symbol = nullptr;
+    cudaDriverEntryPointQueryResult query{};
+    const cudaError_t e =
+        cudaGetDriverEntryPoint("cuPointerGetAttribute", &symbol, cudaEnableDefault, &query);
+    if (e != cudaSuccess || query != cudaDriverEntryPointSuccess) return PointerAttributeFn{nullptr};
+    return reinterpret_cast<PointerAttributeFn>(symbol);
+  }();
+  return fn;
+}
+
+}  // namespace
+
 void RequireOnDevice(const void* pointer, const char* name) {
   int device = 0;
   Check(cudaGetDevice(&device), "cudaGetDevice");
-  cudaPointerAttributes attr{};
+  int owner = -1;
+  const PointerAttributeFn query = GetPointerAttribute();
+  if (query != nullptr &&
+      query(&owner, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL,
+            reinterpret_cast<CUdeviceptr>(pointer)) == CUDA_SUCCESS &&
+      owner == device)
+    return;
+  cudaPointerAttributes attr{};  // another device's, unified or host memory
   Check(cudaPointerGetAttributes(&attr, pointer), "pointer attributes");
   if (attr.type == cudaMemoryTypeUnregistered ||
       (attr.type == cudaMemoryTypeDevice && attr.device != device))
