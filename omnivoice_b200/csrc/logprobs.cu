@@ -196,6 +196,10 @@ struct Row<float> {
     for (int i = 0; i < kN; ++i) mask |= At(q, i) > x ? 1u << i : 0u;
     return mask;
   }
+  // Value i, i not known when compiling.
+  static __device__ __forceinline__ float Pick(const uint4& q, int i) {
+    return __uint_as_float(i < 2 ? (i == 0 ? q.x : q.y) : (i == 2 ? q.z : q.w));
+  }
   // The greatest value below x.
   static __device__ __forceinline__ float Below(float x) {
     return __uint_as_float(x > 0.0f ? __float_as_uint(x) - 1
@@ -254,6 +258,10 @@ struct Row<__half> {
     const uint32_t m = (__hgt2_mask(Pair(q.x), h) & 0x00020001u) | (__hgt2_mask(Pair(q.y), h) & 0x00080004u) |
                        (__hgt2_mask(Pair(q.z), h) & 0x00200010u) | (__hgt2_mask(Pair(q.w), h) & 0x00800040u);
     return (m | (m >> 16)) & 0xFFu;
+  }
+  static __device__ __forceinline__ float Pick(const uint4& q, int i) {
+    const uint32_t w = i < 4 ? (i < 2 ? q.x : q.y) : (i < 6 ? q.z : q.w);
+    return __half2float(__ushort_as_half(static_cast<uint16_t>(w >> (i & 1) * 16)));
   }
   static __device__ __forceinline__ float Below(float x) {
     const uint16_t h = __half_as_ushort(__float2half_rn(x));
@@ -432,17 +440,19 @@ __device__ __forceinline__ void Rebase(RowStats& s, float m) {
   }
   s.m = m;
 }
+// The whole warp's sums, in all lanes; in a fixed order.
 template <typename T>
-__device__ __forceinline__ void Merge(RowStats& s, RowStats o) {
-  const float top = MaxNan(s.m, o.m);
+__device__ __forceinline__ void MergeWarp(RowStats& s) {
+  float top = s.m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = MaxNan(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
   if (!(fabsf(top) < INFINITY)) {  // nothing yet, or no distribution
     s.m = top;
     return;
   }
   Rebase<T>(s, top);
-  Rebase<T>(o, top);
-  s.z += o.z;
-  s.w += o.w;
+  s.z = warp_sum(s.z);
+  s.w = warp_sum(s.w);
 }
 
 __device__ __forceinline__ uint32_t LoadCluster32(uint32_t address) {
@@ -469,26 +479,27 @@ struct LongShared {
   float threshold;
 };
 
-// Leaves the top_k greatest of the `count` keys in order in keys[0 ..) and
-// sets count and threshold.  Every thread calls it, after a barrier.
-__device__ __forceinline__ void Prune(LongShared& s, int k) {
+// Leaves the top_k greatest of the keys in order in keys[0 ..) and sets count
+// and threshold; `slots` slots hold `present` keys, the others 0.  Every
+// thread calls it, after a barrier.
+__device__ __forceinline__ void Prune(LongShared& s, int k, int slots, int present) {
   // Four lanes count the keys ahead of one.
-  const int n = s.count, lanes = threadIdx.x & 3;
-  for (int i0 = 0; i0 < n; i0 += kThreads / 4) {
+  const int lanes = threadIdx.x & 3;
+  for (int i0 = 0; i0 < slots; i0 += kThreads / 4) {
     const int i = i0 + (threadIdx.x >> 2);
-    const uint64_t key = i < n ? s.keys[i] : 0;
+    const uint64_t key = i < slots ? s.keys[i] : 0;
     int r = 0;
 #pragma unroll 4
-    for (int j = lanes; j < n; j += 4) r += s.keys[j] > key ? 1 : 0;
+    for (int j = lanes; j < slots; j += 4) r += s.keys[j] > key ? 1 : 0;
     r += __shfl_xor_sync(0xFFFFFFFFu, r, 1);
     r += __shfl_xor_sync(0xFFFFFFFFu, r, 2);
-    if (i < n && lanes == 0 && r < k) s.sorted[r] = key;
+    if (key != 0 && lanes == 0 && r < k) s.sorted[r] = key;
   }
   __syncthreads();
-  if (static_cast<int>(threadIdx.x) < min(n, k)) s.keys[threadIdx.x] = s.sorted[threadIdx.x];
-  if (threadIdx.x == 0) {
-    s.count = min(n, k);
-    s.threshold = n >= k ? KeyValue(s.sorted[k - 1]) : -INFINITY;
+  if (static_cast<int>(threadIdx.x) < min(present, k)) s.keys[threadIdx.x] = s.sorted[threadIdx.x];
+  if (threadIdx.x == 32) {
+    s.count = min(present, k);
+    s.threshold = present >= k ? KeyValue(s.sorted[k - 1]) : -INFINITY;
   }
   __syncthreads();
 }
@@ -601,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, 4)
       }
       __syncthreads();
     } else {
-      Prune(s, k);
+      Prune(s, k, s.count, s.count);
     }
   };
   if (part == 0) {
@@ -672,19 +683,30 @@ __global__ void __launch_bounds__(kThreads, 4)
       threshold = s.threshold;
     }
     if (top > threshold) {
+      uint32_t masks[kVectors];
+      int n = 0;
 #pragma unroll
       for (int u = 0; u < kVectors; ++u) {
-        uint32_t mask = R::MaskAbove(q[u], threshold);
+        masks[u] = R::MaskAbove(q[u], threshold);
+        n += __popc(masks[u]);
+      }
+      int at = atomicAdd(&s.count, n);
+#pragma unroll
+      for (int u = 0; u < kVectors; ++u) {
+        uint32_t mask = masks[u];
         const int j = head + (v0 + u * kThreads + tid) * kE;
         while (mask != 0) {
           const int e = __ffs(mask) - 1;
           mask &= mask - 1;
-          push(ToFloat(src[j + e]), j + e);
+          if (at < kKeys) s.keys[at] = AlternativeKey(R::Pick(q[u], e), j + e);
+          ++at;
         }
       }
     }
-    // After chunks 1, 2, 4, 8, ...: about top_k values pass in between.
-    if ((chunk & (chunk + 1)) == 0) {
+    // After chunks 1, 2, 4, 8, ...: about top_k values pass in between.  Over
+    // 512 half rows of 151,936 values this took 61 us, settling after every
+    // chunk 70 us and after chunks 1, 4, 16, ... 79 us.
+    if ((chunk & (chunk + 1)) == 0 && v0 + kStep < end) {
       const int high = head + min(end, v0 + kStep) * kE;
       settle(settled, high);
       settled = high;
@@ -694,15 +716,8 @@ __global__ void __launch_bounds__(kThreads, 4)
   if (row_end && head + vectors * kE + tid < a.vocab) scalar(head + vectors * kE + tid, s.threshold);
   if (k > 0) settle(settled, row_end ? a.vocab : head + end * kE);
 
-  // The CTA's sums, in a fixed order.
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    RowStats other;
-    other.m = __shfl_xor_sync(0xFFFFFFFFu, st.m, o);
-    other.z = __shfl_xor_sync(0xFFFFFFFFu, st.z, o);
-    other.w = __shfl_xor_sync(0xFFFFFFFFu, st.w, o);
-    Merge<T>(st, other);
-  }
+  // The CTA's sums.
+  MergeWarp<T>(st);
   ahead = __reduce_add_sync(0xFFFFFFFFu, ahead);
   if (lane == 0) {
     s.stats[warp] = st;
@@ -716,14 +731,7 @@ __global__ void __launch_bounds__(kThreads, 4)
       total = s.stats[lane];
       sum = s.ahead[lane];
     }
-#pragma unroll
-    for (int o = kThreads / 64; o > 0; o >>= 1) {
-      RowStats other;
-      other.m = __shfl_xor_sync(0xFFFFFFFFu, total.m, o);
-      other.z = __shfl_xor_sync(0xFFFFFFFFu, total.z, o);
-      other.w = __shfl_xor_sync(0xFFFFFFFFu, total.w, o);
-      Merge<T>(total, other);
-    }
+    MergeWarp<T>(total);
     sum = __reduce_add_sync(0xFFFFFFFFu, sum);
     if (lane == 0) {
       s.total = total;
@@ -734,36 +742,41 @@ __global__ void __launch_bounds__(kThreads, 4)
     __syncthreads();
     cluster_sync();
     if (part == 0) {
-      // The other parts' alternatives behind this one's; their sums in part
-      // order.  Parts hold ascending indices, and the keys order ties.
-      if (k > 0) {
-        for (int i = tid; i < (cluster - 1) * kMaxTopK; i += kThreads) {
-          const int peer = 1 + i / kMaxTopK, at = i % kMaxTopK;
-          const int n = static_cast<int>(LoadCluster32(mapa_shared(smem_u32(&s.count), peer)));
-          uint64_t key = 0;
-          if (at < n) key = LoadCluster64(mapa_shared(smem_u32(&s.keys[at]), peer));
-          s.sorted[i] = key;
+      if (warp == 0) {  // lane p: part p's sums
+        RowStats total = {-INFINITY, 0.0f, 0.0f};
+        int sum = 0;
+        if (lane < cluster) {
+          const uint32_t at = mapa_shared(smem_u32(&s.total), lane);
+          total.m = __uint_as_float(LoadCluster32(at));
+          total.z = __uint_as_float(LoadCluster32(at + 4));
+          total.w = __uint_as_float(LoadCluster32(at + 8));
+          sum = static_cast<int>(LoadCluster32(mapa_shared(smem_u32(&s.total_ahead), lane)));
         }
-        __syncthreads();
-        for (int i = tid; i < (cluster - 1) * kMaxTopK; i += kThreads)
-          if (s.sorted[i] != 0) s.keys[atomicAdd(&s.count, 1)] = s.sorted[i];
-        __syncthreads();
-        Prune(s, k);
+        MergeWarp<T>(total);
+        sum = __reduce_add_sync(0xFFFFFFFFu, sum);
+        __syncwarp();
+        if (lane == 0) {
+          s.total = total;
+          s.total_ahead = sum;
+        }
       }
-      if (tid == 0) {
-        RowStats total = s.total;
-        int sum = s.total_ahead;
-        for (int peer = 1; peer < cluster; ++peer) {
-          const uint32_t at = mapa_shared(smem_u32(&s.total), peer);
-          RowStats o;
-          o.m = __uint_as_float(LoadCluster32(at));
-          o.z = __uint_as_float(LoadCluster32(at + 4));
-          o.w = __uint_as_float(LoadCluster32(at + 8));
-          Merge<T>(total, o);
-          sum += static_cast<int>(LoadCluster32(mapa_shared(smem_u32(&s.total_ahead), peer)));
+      // The other parts' alternatives behind this one's.  Parts hold ascending
+      // indices, and the keys order ties.
+      if (k > 0) {
+        const int own = s.count, others = (cluster - 1) * k;
+        int found = 0;
+        for (int i0 = 0; i0 < others; i0 += kThreads) {  // the same turns for all threads
+          const int i = i0 + tid, peer = 1 + i / k, at = i % k;
+          uint64_t key = 0;
+          if (i < others) {
+            const int n = static_cast<int>(LoadCluster32(mapa_shared(smem_u32(&s.count), peer)));
+            key = LoadCluster64(mapa_shared(smem_u32(&s.keys[at]), peer));
+            if (at >= n) key = 0;
+            s.keys[own + i] = key;
+          }
+          found += __syncthreads_count(key != 0);
         }
-        s.total = total;
-        s.total_ahead = sum;
+        Prune(s, k, own + others, own + found);
       }
     }
     __syncthreads();
@@ -816,7 +829,8 @@ void LaunchLogprobs(const LogprobArgs& a, cudaStream_t stream) {
     return;
   }
   // Few rows: up to eight CTAs of a cluster share one, as long as each has
-  // vectors for all of its threads.
+  // vectors for all of its threads (one row of 151,936 floats: 17.5 us with
+  // eight, 19.6 us with sixteen, which end later at their cluster barriers).
   unsigned cluster = 1;
   while (cluster < 8 && items * cluster * 2 <= 2 * SmCount() &&
          a.vocab >= static_cast<int>(cluster) * 2 * kThreads * Row<T>::kN)
