@@ -1053,10 +1053,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const CacheView& cache = a.cache;
   pdl_trigger();
   pdl_wait();
-  const int kv_head = blockIdx.z, seq = blockIdx.y;
+  // Heads first: CTAs that run together read whole rows of q and whole pages.
   // The last row tiles of a causal sequence see most: they start first.
-  const int tile = args.tiles - 1 - static_cast<int>(blockIdx.x) / args.splits;
-  const int split = static_cast<int>(blockIdx.x) % args.splits;
+  const int kv_head = static_cast<int>(blockIdx.x) % cache.kv_heads, seq = blockIdx.y;
+  const int part_of_rows = static_cast<int>(blockIdx.x) / cache.kv_heads;
+  const int tile = args.tiles - 1 - part_of_rows / args.splits;
+  const int split = part_of_rows % args.splits;
   const RowSpan span = SequenceRows(a.cu_rows, seq, a.rows, a.max_rows, a.err);
   const int rows = span.count * a.group.d;  // at most 2^31 (host check)
   const int row0 = tile * args.tile_rows;
@@ -1580,8 +1582,8 @@ int ov_attention_kv_cache(const ov_kv_cache* cache, const uint16_t* q, size_t ld
                "max_length exceeds the page table");
     OV_REQUIRE(ld_q % 8 == 0 && ld_q >= heads * kCacheHeadDim, "q stride");
     OV_REQUIRE(ld_out % 8 == 0 && ld_out >= heads * kCacheHeadDim, "out stride");
-    OV_REQUIRE(std::min(max_rows, rows) <= ((size_t{1} << 31) - 512) / (heads / cache->kv_heads),
-               "max_rows * heads / kv_heads must stay below 2^31");
+    OV_REQUIRE(std::min(max_rows, rows) <= ((size_t{1} << 31) - 512) / heads,
+               "max_rows * heads must stay below 2^31");
     if (rows == 0 || max_rows == 0 || c.num_seqs == 0) return;
     RequireAligned(q, 16, "q");
     RequireAligned(out, 16, "out");
@@ -1643,8 +1645,8 @@ int ov_attention_kv_cache(const ov_kv_cache* cache, const uint16_t* q, size_t ld
     SetMaxDynamicSmem(reinterpret_cast<const void*>(cache_attention_tile_kernel),
                       static_cast<int>(kTileSmem));
     Launch(cache_attention_tile_kernel,
-           dim3(static_cast<unsigned>(args.tiles) * static_cast<unsigned>(args.splits),
-                static_cast<unsigned>(c.num_seqs), static_cast<unsigned>(c.kv_heads)),
+           dim3(static_cast<unsigned>(args.tiles) * static_cast<unsigned>(args.splits * c.kv_heads),
+                static_cast<unsigned>(c.num_seqs)),
            dim3(kTileThreads), kTileSmem, AsStream(stream), "cache attention kernel launch", map_k,
            map_v, args);
   });
