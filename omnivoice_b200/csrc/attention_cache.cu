@@ -1442,12 +1442,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     named_barrier(1, 256);
     if (!s.last) return;
     const float* base_part = args.parts + item * args.splits * TilePartFloats(args.tile_rows);
-    for (int i = tid; i < 8 * args.tile_rows; i += 256) {
-      const int row = i & (args.tile_rows - 1), d16 = i / args.tile_rows;  // 16 columns of a row
-      if (row >= here) continue;
+    for (int i = tid; i < 8 * here; i += 256) {
+      const int d16 = i / here, row = i - d16 * here;  // 16 columns of a row
       float top = -INFINITY, sum = 0.0f;
       float o[16] = {};
-#pragma unroll 2
+#pragma unroll 4
       for (int x = 0; x < parts; ++x) {
         const float* p = base_part + x * TilePartFloats(args.tile_rows);
         const float2 ms = __ldcg(reinterpret_cast<const float2*>(p + stats_at + 2 * row));
