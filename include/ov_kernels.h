@@ -215,7 +215,8 @@ int ov_attention_varlen_items(const uint16_t* qkv, size_t ld_qkv, size_t rows,
  *
  * A page holds `page_tokens` consecutive tokens of one sequence; per page and
  * kv head it has int8 codes [page_tokens][head_dim] and one float32 scale,
- * for keys and for values apart.  A code c stands for c * scale.  Token t of
+ * for keys and for values apart (not negative; NaN makes the page's values
+ * NaN).  A code c stands for c * scale.  Token t of
  * sequence s lies in page page_table[s * max_pages + t / page_tokens], slot
  * t % page_tokens.  Sequences may share pages that they only read.
  * All arrays are DEVICE memory; the struct itself is read during the call.
@@ -296,8 +297,9 @@ int ov_kv_cache_read(const ov_kv_cache* cache, const int32_t* cu_rows, const int
  * are joined in a fixed order: results do not depend on timing.  That needs
  * `workspace` (16-byte aligned) of ov_attention_kv_cache_workspace_bytes;
  * with a smaller one or NULL each row runs on one CTA.  Zero it once before
- * its first use (every call leaves its counters zero); calls sharing a
- * workspace must not overlap, captured ones included. */
+ * its first use: every call leaves its counters zero, so calls of any shapes
+ * may share a workspace that is large enough for each.  Calls sharing one
+ * must not overlap, captured ones included. */
 int ov_attention_kv_cache(const ov_kv_cache* cache, const uint16_t* q, size_t ld_q, size_t rows,
                           const int32_t* cu_rows, size_t max_rows, const int32_t* lengths,
                           size_t max_length, size_t heads, int causal, float scale, uint16_t* out,

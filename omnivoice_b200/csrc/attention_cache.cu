@@ -122,7 +122,7 @@ struct alignas(16) SlotInfo {
 
 struct StreamArgs {
   CacheAttnArgs a;
-  uint32_t* counters;  // one for each (sequence, kv head); null: no item is split
+  uint32_t* counters;  // of the item that goes on behind each CTA; null: no item is split
   float* parts;        // [CTA][2][JoinFloats(join_rows)]: of the item begun before, of the last
   int join_rows;       // rows of a (sequence, kv head) at most
 };
@@ -173,10 +173,12 @@ __device__ __forceinline__ int load_early(const int32_t* p) {
   return v;
 }
 
-// Factor of a key scale in the exponent; a page of zeros has scale 0 and
-// scores 0, which any finite factor keeps.
+// Factor of a key scale in the exponent.  Not 0, which would make NaN of a
+// hidden score's -inf: a page of zeros has scale 0 and scores 0, which any
+// finite factor keeps, and scores that a smaller one tells apart are equal.
 __device__ __forceinline__ float KeyFactor(float scale, float scale_log2) {
-  return scale == 0.0f ? 1.0f : scale * scale_log2;
+  const float factor = scale * scale_log2;
+  return factor >= 0.0f && factor < 0x1.0p-126f ? 0x1.0p-126f : factor;
 }
 // Adds a part's maximum and sum (ms) to a row's; returns the factors of the
 // O so far and of the part's O.
@@ -797,8 +799,9 @@ __global__ void __launch_bounds__(kStreamThreads + 128, 1)
   const int64_t cta_width = width * kStreamWarps;
   if (tid < 2 && shared.has[tid] != 0) {
     const ItemAt it = shared.part[tid];
-    const int64_t parts = Divide(it.end() - 1, cta_width) - Divide(it.begin, cta_width);
-    uint32_t* counter = args.counters + static_cast<int64_t>(it.seq) * cache.kv_heads + it.head;
+    const int64_t first = Divide(it.begin, cta_width);  // at most one item goes on behind a CTA
+    const int64_t parts = Divide(it.end() - 1, cta_width) - first;
+    uint32_t* counter = args.counters + first;
     const bool last = atom_add_acq_rel(counter, 1u) == static_cast<uint32_t>(parts);
     if (last) *counter = 0;
     shared.last[tid] = last;
@@ -1475,12 +1478,21 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   }
 }
 
+// A workspace begins with counters, as many for every shape, so that calls of
+// different shapes can share it: none finds another's parts in their place.
+constexpr size_t kCounterBytes = 4096;
+
+// CTAs of a call that splits items (each may need a counter).
+size_t SplitCtas() {
+  return std::min<size_t>(static_cast<size_t>(SmCount()), kCounterBytes / sizeof(uint32_t));
+}
+
 // How a call runs: the streaming kernel's rows for a (sequence, kv head), its
 // CTAs and the scratch that splitting takes.
 struct StreamPlan {
   int rows;       // 0: too many for it
   unsigned ctas;
-  size_t counter_bytes, part_bytes;
+  size_t part_bytes;
 };
 
 StreamPlan PlanStream(const ov_kv_cache* cache, size_t max_rows, size_t max_length, size_t heads) {
@@ -1492,8 +1504,7 @@ StreamPlan PlanStream(const ov_kv_cache* cache, size_t max_rows, size_t max_leng
   const size_t units = std::max<size_t>(1, (max_length + kUnit - 1) / kUnit);
   const size_t least = kMinUnits * kStreamWarps;
   plan.ctas = static_cast<unsigned>(
-      std::min<size_t>(SmCount(), items * ((units + least - 1) / least)));
-  plan.counter_bytes = (items * sizeof(uint32_t) + 15) / 16 * 16;
+      std::min(SplitCtas(), items * ((units + least - 1) / least)));
   plan.part_bytes = 2 * plan.ctas * JoinFloats(plan.rows) * sizeof(float);
   return plan;
 }
@@ -1501,14 +1512,14 @@ StreamPlan PlanStream(const ov_kv_cache* cache, size_t max_rows, size_t max_leng
 // The tile kernel's CTAs and scratch.
 struct TilePlan {
   int tile_rows, tiles, splits;
-  size_t counter_bytes, part_bytes;
+  size_t part_bytes;
 };
 
 TilePlan PlanTiles(const ov_kv_cache* cache, size_t max_rows, size_t max_length, size_t heads) {
   TilePlan plan{};
   const size_t rows = max_rows * (heads / cache->kv_heads);
   const size_t pairs = cache->num_seqs * cache->kv_heads;  // of sequence and kv head
-  const size_t sms = static_cast<size_t>(SmCount());
+  const size_t sms = SplitCtas();
   // Single tiles while they all fit the GPU at once, else tile pairs.
   plan.tile_rows = (rows + kQ - 1) / kQ * pairs <= sms ? kQ : 2 * kQ;
   plan.tiles = static_cast<int>((rows + plan.tile_rows - 1) / plan.tile_rows);
@@ -1516,10 +1527,8 @@ TilePlan PlanTiles(const ov_kv_cache* cache, size_t max_rows, size_t max_length,
   const size_t key_tiles = (max_length + kKeys - 1) / kKeys;
   plan.splits = static_cast<int>(
       std::max<size_t>(1, std::min(sms / items, key_tiles / kMinKeyTiles)));
-  if (plan.splits > 1) {
-    plan.counter_bytes = (items * sizeof(uint32_t) + 15) / 16 * 16;
+  if (plan.splits > 1)
     plan.part_bytes = items * plan.splits * TilePartFloats(plan.tile_rows) * sizeof(float);
-  }
   return plan;
 }
 
@@ -1556,12 +1565,10 @@ size_t ov_attention_kv_cache_workspace_bytes(const ov_kv_cache* cache, size_t ro
     OV_REQUIRE(heads > 0 && heads % cache->kv_heads == 0, "heads must be a multiple of kv_heads");
     if (std::min(max_rows, rows) == 0 || cache->num_seqs == 0) return;
     const StreamPlan plan = PlanStream(cache, std::min(max_rows, rows), max_length, heads);
-    if (plan.rows > 0) {
-      bytes = plan.counter_bytes + plan.part_bytes;
-    } else {
-      const TilePlan tiles = PlanTiles(cache, std::min(max_rows, rows), max_length, heads);
-      bytes = tiles.counter_bytes + tiles.part_bytes;
-    }
+    const size_t parts = plan.rows > 0
+                             ? plan.part_bytes
+                             : PlanTiles(cache, std::min(max_rows, rows), max_length, heads).part_bytes;
+    if (parts > 0) bytes = kCounterBytes + parts;
   });
   return status == OV_OK ? bytes : 0;
 }
@@ -1618,9 +1625,9 @@ int ov_attention_kv_cache(const ov_kv_cache* cache, const uint16_t* q, size_t ld
       EncodeCodesMap(&map_v, c.values, cache, box, CU_TENSOR_MAP_SWIZZLE_128B);
       StreamArgs args{a, nullptr, nullptr, plan.rows};
       unsigned ctas = static_cast<unsigned>(c.num_seqs * c.kv_heads);
-      if (workspace != nullptr && workspace_bytes >= plan.counter_bytes + plan.part_bytes) {
+      if (workspace != nullptr && workspace_bytes >= kCounterBytes + plan.part_bytes) {
         args.counters = static_cast<uint32_t*>(workspace);
-        args.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.counter_bytes);
+        args.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
         ctas = plan.ctas;
       }
       if (plan.rows <= 8) LaunchStream<1>(args, ctas, map_k, map_v, AsStream(stream));
@@ -1630,9 +1637,9 @@ int ov_attention_kv_cache(const ov_kv_cache* cache, const uint16_t* q, size_t ld
     TilePlan tiles = PlanTiles(cache, a.max_rows, max_length, heads);
     TileArgs args{a, nullptr, nullptr, tiles.tile_rows, tiles.tiles, tiles.splits};
     if (tiles.splits > 1) {
-      if (workspace != nullptr && workspace_bytes >= tiles.counter_bytes + tiles.part_bytes) {
+      if (workspace != nullptr && workspace_bytes >= kCounterBytes + tiles.part_bytes) {
         args.counters = static_cast<uint32_t*>(workspace);
-        args.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + tiles.counter_bytes);
+        args.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
       } else {
         args.splits = 1;
       }

@@ -407,6 +407,108 @@ def test_a_nan_page_reaches_its_own_sequence_and_head_only(n):
         assert got[n:, 2 * D:].isnan().all()
 
 
+@pytest.mark.parametrize("seqs,heads,kv", [(33, 4, 2), (64, 8, 8), (300, 2, 1), (1000, 1, 1)])
+@pytest.mark.parametrize("n", [1, 9])
+def test_many_sequences(seqs, heads, kv, n):
+    """More sequences than lanes, some without rows or tokens."""
+    g = torch.Generator().manual_seed(seqs)
+    lengths = [int(x) for x in torch.randint(0, 90, (seqs,), generator=g)]
+    counts = [int(x) for x in torch.randint(0, n + 1, (seqs,), generator=g)]
+    lengths[7], counts[7] = 1500, n
+    check_attention(filled(seqs, 32, kv, lengths, g), counts, lengths, heads, True, g)
+
+
+@pytest.mark.parametrize("n", [4, 60])
+@pytest.mark.parametrize("which", [0, 1])
+def test_a_nan_page_that_only_later_rows_see(n, which):
+    g = torch.Generator().manual_seed(n)
+    length = 64 + n // 2  # half of the rows end before the second page
+    ref = filled(1, 64, 1, [length], g)
+    ref.scales[which][int(ref.table[0, 1]), 0] = float("nan")
+    q = torch.randn(n, 2 * D, generator=g).half()
+    gpu = GpuCache(ref)
+    out = torch.zeros(n, 2 * D, dtype=torch.float16, device="cuda")
+    gpu.attend(q.cuda(), [n], [length], 2, True, 0.1, out, gpu.workspace(n, n, length, 2))
+    got = out.cpu()
+    clean = 64 - (length - n)  # rows that see the first page only
+    assert got[clean:].isnan().all()
+    ref.scales[which][int(ref.table[0, 1]), 0] = 0.01  # not seen by these
+    want, bound = reference(ref, q, [n], [length], 2, True, 0.1)
+    assert ((got[:clean].double() - want[:clean]).abs() <= bound[:clean]).all()
+
+
+@pytest.mark.parametrize("n", [1, 50])
+def test_sequences_that_share_pages(n):
+    g = torch.Generator().manual_seed(n)
+    lengths = [200, 230, 130]
+    ref = filled(3, 64, 2, lengths, g)
+    ref.table[1, :2] = ref.table[0, :2]
+    ref.table[2, :2] = ref.table[0, :2]
+    check_attention(ref, [n] * 3, lengths, 4, False, g)
+
+
+@pytest.mark.parametrize("n", [2, 30])
+def test_the_least_scales(n):
+    """Factors that underflow: every score is 0, hidden tokens stay hidden."""
+    g = torch.Generator().manual_seed(n)
+    ref = filled(1, 32, 1, [100], g)
+    for s in ref.scales:
+        s.copy_(torch.where(s.isnan(), s, 1e-6))
+    check_attention(ref, [n], [100], 2, True, g, scale=1e-36)
+    ref.scales[0].copy_(torch.where(ref.scales[0].isnan(), ref.scales[0], 1e-38))
+    check_attention(ref, [n], [100], 2, True, g, scale=1e-30)
+
+
+def test_one_workspace_for_calls_of_any_shape_and_two_graphs():
+    """A workspace goes from single tokens of few sequences to many, to
+    blocks of rows and back, eagerly and in two graphs that share it."""
+    g = torch.Generator().manual_seed(4)
+    shapes = [([3000], [1], 4, 2), ([700] * 40, [1] * 40, 4, 4), ([2500], [30], 8, 1),
+              ([900, 900], [100, 3], 2, 2), ([3000], [2], 4, 1)]
+    calls, need = [], 0
+    for lengths, counts, heads, kv in shapes:
+        gpu = GpuCache(filled(len(lengths), 32, kv, lengths, g))
+        q = torch.randn(sum(counts), heads * D, generator=g).half().cuda()
+        own = gpu.workspace(sum(counts), max(counts), max(lengths), heads)
+        need = max(need, own.numel())
+        want = gpu.attend(q, counts, lengths, heads, True, 0.1, torch.zeros_like(q), own)
+        calls.append((gpu, q, counts, lengths, heads, want))
+    torch.cuda.synchronize()
+    shared = torch.zeros(need, dtype=torch.uint8, device="cuda")
+    for _ in range(3):
+        for gpu, q, counts, lengths, heads, want in calls:
+            got = gpu.attend(q, counts, lengths, heads, True, 0.1, torch.zeros_like(q), shared)
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+    lib, s = N.lib(), torch.cuda.Stream()
+    graphs, outs, held = [], [], []
+    for part in (calls[:3], calls[2:]):
+        prepared = [(gpu, q, i32(cumulative(counts)), i32(lengths), counts, lengths, heads,
+                     torch.zeros_like(q)) for gpu, q, counts, lengths, heads, _ in part]
+        torch.cuda.synchronize()
+        graph = ctypes.c_void_p()
+        N.check(lib.ov_graph_capture_begin(s.cuda_stream))
+        for gpu, q, cu, ln, counts, lengths, heads, out in prepared:
+            N.check(lib.ov_attention_kv_cache(
+                ctypes.byref(gpu.desc), q.data_ptr(), q.stride(0), q.shape[0], cu.data_ptr(),
+                max(counts), ln.data_ptr(), max(lengths), heads, 1, 0.1, out.data_ptr(),
+                out.stride(0), shared.data_ptr(), shared.numel(), s.cuda_stream))
+        N.check(lib.ov_graph_capture_end(s.cuda_stream, ctypes.byref(graph)))
+        graphs.append(graph)
+        outs.append([p[-1] for p in prepared])
+        held.append(prepared)
+    for turn in (0, 1, 1, 0):
+        for out in outs[turn]:
+            out.zero_()
+        torch.cuda.synchronize()
+        N.check(lib.ov_graph_launch(graphs[turn], s.cuda_stream))
+        torch.cuda.synchronize()
+        for out, call in zip(outs[turn], (calls[:3], calls[2:])[turn]):
+            assert torch.equal(out, call[5])
+    for graph in graphs:
+        N.check(lib.ov_graph_destroy(graph))
+
+
 @pytest.mark.parametrize("n", [1, 40])
 def test_bad_pages_and_lengths_are_skipped_and_reported(n):
     """A page outside the cache counts as tokens that nothing sees."""
@@ -527,3 +629,66 @@ def test_another_stream_and_graph_replay():
         ends += 1
         torch.cuda.synchronize()
     N.check(lib.ov_graph_destroy(graph))
+
+
+def test_a_decoding_step_next_to_the_varlen_attention():
+    """Projection with QK norm and RoPE, cache, attention, head and log
+    probabilities as a caller chains them; the attention is within what
+    rounding keys and values to a page's grid can change of the one that
+    ov_attention_varlen computes from the same rows."""
+    g = torch.Generator().manual_seed(11)
+    heads, kv, width, n, page = 4, 2, 256, 150, 32
+    cols = (heads + 2 * kv) * D
+    lib = N.lib()
+    x = torch.randn(n, width, generator=g).half().cuda()
+    w = (torch.randn(cols, width, generator=g) / 16).half().cuda()
+    norm = torch.ones(D, device="cuda")
+    cos = torch.ones(n, D // 2, device="cuda")
+    sin = torch.zeros(n, D // 2, device="cuda")
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    args = N.EpilogueArgs(q_norm=norm.data_ptr(), k_norm=norm.data_ptr(), positions=pos.data_ptr(),
+                          rope_cos=cos.data_ptr(), rope_sin=sin.data_ptr(), max_positions=n,
+                          heads=heads, kv_heads=kv, head_dim=D, epsilon=1e-6)
+    qkv = torch.empty(n, cols, dtype=torch.float16, device="cuda")
+    N.check(lib.ov_gemm_f16(x.data_ptr(), width, w.data_ptr(), qkv.data_ptr(), cols, n, width, cols,
+                            N.OV_EPI_QKNORM_ROPE_F16, ctypes.byref(args), None, 0, stream()))
+    plain = torch.empty(n, heads * D, dtype=torch.float16, device="cuda")
+    cu = i32([0, n])
+    N.check(lib.ov_attention_varlen(qkv.data_ptr(), cols, n, cu.data_ptr(), 1, n, heads, kv, D,
+                                    D ** -0.5, plain.data_ptr(), heads * D, stream()))
+    gpu = GpuCache(Cache(5, page, kv, torch.tensor([[3, 0, 2, 4, 1]])))
+    k, v = qkv[:, heads * D:(heads + kv) * D], qkv[:, (heads + kv) * D:]
+    gpu.write(k, v, [n], [0])
+    out = torch.empty_like(plain)
+    gpu.attend(qkv[:, :heads * D], [n], [n], heads, False, D ** -0.5, out, gpu.workspace(n, n, n, heads))
+    last = torch.empty(1, heads * D, dtype=torch.float16, device="cuda")
+    gpu.attend(qkv[n - 1:, :heads * D], [1], [n], heads, True, D ** -0.5, last, gpu.workspace(1, 1, n, heads))
+    torch.cuda.synchronize()
+    # Half a step of at most amax / 127 for a value, and for a key through
+    # |q|_1 * step / 2 * scale in each score (a relative change of twice its
+    # exponential); halves elsewhere.
+    step_k = float(k.abs().max()) / 127
+    step_v = float(v.abs().max()) / 127
+    shift = float(qkv[:, :heads * D].float().view(n, heads, D).abs().sum(-1).max()) * step_k / 2 * D ** -0.5
+    bound = step_v / 2 + float(v.abs().max()) * (torch.tensor(2 * shift).expm1().item() + 2.0 ** -9)
+    assert float((out - plain).abs().max()) <= bound
+    assert float((last - plain[n - 1:]).abs().max()) <= bound
+    # The audio head over the attention's output, four codebooks.
+    books, vocab = 4, 1025
+    head = (torch.randn(books * vocab, heads * D, generator=g) / 8).half().cuda()
+    logits = torch.empty(n, books * vocab + 12, device="cuda")
+    N.check(lib.ov_gemm_f16(out.data_ptr(), heads * D, head.data_ptr(), logits.data_ptr(),
+                            logits.stride(0), n, heads * D, books * vocab, N.OV_EPI_STORE_F32, None,
+                            None, 0, stream()))
+    targets = torch.randint(0, vocab, (books, n), generator=g).to(torch.int32).cuda()
+    lp = torch.empty(books, n, device="cuda")
+    rank = torch.empty(books, n, dtype=torch.int32, device="cuda")
+    N.check(lib.ov_token_logprobs(logits.data_ptr(), N.OV_LOGITS_F32, logits.stride(0), n, books,
+                                  vocab, targets.data_ptr(), 0, lp.data_ptr(), None,
+                                  rank.data_ptr(), None, None, stream()))
+    torch.cuda.synchronize()
+    z = logits[:, :books * vocab].unflatten(1, (books, vocab)).transpose(0, 1)
+    t = targets.long()[..., None]
+    want = torch.log_softmax(z.double(), -1).gather(2, t)[..., 0]
+    assert float((lp.double() - want).abs().max()) <= 1e-5 * (1 + float(want.abs().max()))
+    assert torch.equal(rank.long(), (z > z.gather(2, t)).sum(-1))

@@ -142,6 +142,34 @@ def test_rows_that_crowd_the_alternatives(vocab, kind):
             check(x.half(), 1, vocab, targets, k)
 
 
+@pytest.mark.parametrize("vocab", [1025, 5000, 30000])
+@pytest.mark.parametrize("half", [False, True])
+def test_masks_of_the_types_lowest_value(vocab, half):
+    """Closed with the lowest finite value instead of -inf: no probability
+    (beside an open token), but a value of its own; and rows of it alone."""
+    g = torch.Generator().manual_seed(vocab)
+    t = torch.float16 if half else torch.float32
+    lowest = torch.finfo(t).min
+    x = torch.randn(5, vocab, generator=g).to(t)
+    x[0, ::2] = lowest
+    x[1] = lowest
+    x[2] = lowest
+    x[2, vocab // 2] = 3.0
+    x[3] = -math.inf
+    x[3, 5::7] = lowest
+    x[4, 3::5] = lowest
+    x[4, 1::5] = -math.inf
+    targets = torch.tensor([[2, 5, vocab // 2, 12, 1]])
+    got = run(x.cuda(), 1, vocab, targets, 9)
+    for r in range(5):
+        lp, rank, entropy, ids, tops = logprobs(x[r], int(targets[0, r]), 9)
+        assert got["rank"][0, r] == rank and got["ids"][0, r].tolist() == ids
+        for mine, true in [(float(got["logprob"][0, r]), lp), *zip(got["tops"][0, r].tolist(), tops)]:
+            # A sum of equal terms as large as their logarithm's rounding.
+            assert mine == true or abs(mine - true) <= 2e-5 + abs(true) * 2.0 ** -21
+        assert abs(float(got["entropy"][0, r]) - entropy) <= 1e-4
+
+
 @pytest.mark.parametrize("vocab", [100, 1025, 5000, 30000])
 def test_rows_without_a_distribution(vocab):
     g = torch.Generator().manual_seed(vocab)
