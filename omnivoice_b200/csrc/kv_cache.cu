@@ -7,7 +7,10 @@
 // with amax over the rows that a page and head take in this call.  The codes
 // are rounded to 8 bits, which is the operator; everything before that is
 // float32.  Both kernels move bytes and nothing else: a written element costs
-// 2 bytes read and 1 written, a read one 1 and 2.
+// 2 bytes read and 1 written, a read one 1 and 2.  Measured on one B200, 8 kv
+// heads: 131,000 tokens written and read back in 272 us (1.62 GB, 5.9 TB/s),
+// the prompts of 64 utterances in 127 us (679 MB, 5.3 TB/s); 64 sequences read
+// in 100 us (535 MB, 5.4 TB/s); one token written and its page read in 6.8 us.
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -143,7 +146,8 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-// Tokens per CTA of the read.
+// Tokens per CTA of the read
+// (64 ragged sequences: 100 us with 16, 122 us with 8, 107 us with 32).
 constexpr int kReadTokens = 16;
 
 __device__ __forceinline__ uint32_t Halves2(uint32_t codes, int byte, float scale) {

@@ -9,6 +9,13 @@
 // each.  Instead of sorting, a threshold that at least top_k values reach is
 // taken from the maxima that the threads hold anyway; the few values that
 // pass it are ranked against one another.
+//
+// Measured on one B200: the audio head's 500 rows of 8 x 1,025 float32 values
+// (16.6 MB) 8.0 us; 512 half rows of 151,936 values (156 MB) with 20
+// alternatives 56 us, 2.8 TB/s: not the reading but about 15 instructions for
+// a value bound it (7.6 for the sums and the rank, the rest for alternatives
+// and what a chunk costs); one float32 row of that length 13.9 us, its
+// clusters' barriers and joins included.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -828,15 +835,21 @@ void LaunchLogprobs(const LogprobArgs& a, cudaStream_t stream) {
            dim3(kWarps * 32), 0, stream, what, a);
     return;
   }
-  // Few rows: up to eight CTAs of a cluster share one, as long as each has
-  // vectors for all of its threads (one row of 151,936 floats: 17.5 us with
-  // eight, 19.6 us with sixteen, which end later at their cluster barriers).
-  unsigned cluster = 1;
-  while (cluster < 8 && items * cluster * 2 <= 2 * SmCount() &&
-         a.vocab >= static_cast<int>(cluster) * 2 * kThreads * Row<T>::kN)
+  // Few rows: up to eight CTAs of a cluster share one, while each has vectors
+  // for all of its threads and they fit the SMs twice over, or, with four
+  // chunks for each and more, four times (an SM holds four).  One row of
+  // 151,936 floats: 13.8 us with eight CTAs, 16 with sixteen; 100 such rows:
+  // 22.3 us with four, 26.1 us with two; 64 rows of 32,000: 10.5 us with four,
+  // 13.7 us with eight.
+  constexpr int kVector = Row<T>::kN;
+  int cluster = 1;
+  while (cluster < 8 && a.vocab >= cluster * 2 * kThreads * kVector) {
+    const bool long_parts = a.vocab >= cluster * 2 * 4 * kThreads * kVectors * kVector;
+    if (items * cluster * 2 > (long_parts ? 4 : 2) * SmCount()) break;
     cluster *= 2;
-  LaunchEx(logprobs_long_kernel<T>, dim3(static_cast<unsigned>(items) * cluster),
-           dim3(kThreads), 0, stream, what, cluster, a, static_cast<int>(cluster));
+  }
+  LaunchEx(logprobs_long_kernel<T>, dim3(static_cast<unsigned>(items * cluster)), dim3(kThreads), 0,
+           stream, what, static_cast<unsigned>(cluster), a, cluster);
 }
 
 }  // namespace
