@@ -9,7 +9,7 @@
 // float32.  Both kernels move bytes and nothing else: a written element costs
 // 2 bytes read and 1 written, a read one 1 and 2.  Measured on one B200, 8 kv
 // heads: 131,000 tokens written and read back in 272 us (1.62 GB, 5.9 TB/s),
-// the prompts of 64 utterances in 127 us (679 MB, 5.3 TB/s); 64 sequences read
+// the prompts of 64 utterances in 122 us (679 MB, 5.6 TB/s); 64 sequences read
 // in 100 us (535 MB, 5.4 TB/s); one token written and its page read in 6.8 us.
 #include <cuda.h>
 #include <cuda_fp16.h>
@@ -59,7 +59,7 @@ __device__ __forceinline__ uint32_t Rescale4(uint32_t codes, float ratio) {
 // in registers (kPage / 16 vectors of 8 halves a thread) between the maximum
 // and the rounding, and memory is read once.
 template <int kPage>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kPage <= 64 ? 8 : 4)
     cache_write_kernel(const CacheView c, const __half* __restrict__ k, int64_t ld_k,
                        const __half* __restrict__ v, int64_t ld_v, int rows,
                        const int32_t* __restrict__ cu_rows, const int32_t* __restrict__ starts,
@@ -89,16 +89,23 @@ __global__ void __launch_bounds__(kThreads)
 
   const int piece = threadIdx.x & 15;  // 8 of the 128 head dimensions
   const int row0 = threadIdx.x >> 4;
-  const __half* src = (value ? v : k) + head * kCacheHeadDim + piece * 8;
   const int64_t ld = value ? ld_v : ld_k;
+  const __half* src = (value ? v : k) + (span.first + (first_token + row0 - start)) * ld +
+                      head * kCacheHeadDim + piece * 8;
+  const bool full = lo == 0 && hi == kPage;
   uint4 x[kVec];
   uint32_t top = 0;  // non-negative halves order as integers, NaN above infinity
+  if (full) {
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) {
-    const int slot = i * 16 + row0;
-    x[i] = make_uint4(0, 0, 0, 0);
-    if (slot >= lo && slot < hi)
-      x[i] = *reinterpret_cast<const uint4*>(src + (span.first + (first_token + slot - start)) * ld);
+    for (int i = 0; i < kVec; ++i, src += 16 * ld)
+      x[i] = *reinterpret_cast<const uint4*>(src);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i, src += 16 * ld) {
+      const int slot = i * 16 + row0;
+      x[i] = make_uint4(0, 0, 0, 0);
+      if (slot >= lo && slot < hi) x[i] = *reinterpret_cast<const uint4*>(src);
+    }
   }
 #pragma unroll
   for (int i = 0; i < kVec; ++i) {
@@ -122,14 +129,15 @@ __global__ void __launch_bounds__(kThreads)
   if (threadIdx.x == 0) scales[scale_at] = scale;
 
   int8_t* dst = (value ? c.values : c.keys) + CacheTile(c, page, head);
+  int8_t* mine = dst + row0 * kCacheHeadDim + piece * 8;
 #pragma unroll
   for (int i = 0; i < kVec; ++i) {
     const int slot = i * 16 + row0;
-    if (slot < lo || slot >= hi) continue;
     uint2 codes;
     codes.x = __byte_perm(Codes2(x[i].x, inverse), Codes2(x[i].y, inverse), 0x5410);
     codes.y = __byte_perm(Codes2(x[i].z, inverse), Codes2(x[i].w, inverse), 0x5410);
-    *reinterpret_cast<uint2*>(dst + slot * kCacheHeadDim + piece * 8) = codes;
+    if (full || (slot >= lo && slot < hi))
+      *reinterpret_cast<uint2*>(mine + i * 16 * kCacheHeadDim) = codes;
   }
   // The kept slots [0, lo) onto the new grid.
   if (lo > 0 && scale > old) {
