@@ -427,7 +427,6 @@ __global__ void __launch_bounds__(kWarps * 32, kPer <= 33 ? 4 : 2)
 
 // ------------------------------ long rows: one CTA, or a cluster, per item
 
-constexpr int kThreads = 256;
 constexpr int kKeys = 1024;      // room for passing values between prunings
 
 // Running maximum, Z = sum 2^t and W = sum 2^t t of what was read, with
@@ -473,6 +472,7 @@ __device__ __forceinline__ uint64_t LoadCluster64(uint32_t address) {
   return v;
 }
 
+template <int kThreads>
 struct LongShared {
   uint64_t keys[kKeys];
   uint64_t sorted[8 * kMaxTopK];
@@ -489,7 +489,8 @@ struct LongShared {
 // Leaves the top_k greatest of the keys in order in keys[0 ..) and sets count
 // and threshold; `slots` slots hold `present` keys, the others 0.  Every
 // thread calls it, after a barrier.
-__device__ __forceinline__ void Prune(LongShared& s, int k, int slots, int present) {
+template <int kThreads>
+__device__ __forceinline__ void Prune(LongShared<kThreads>& s, int k, int slots, int present) {
   // Four lanes count the keys ahead of one.
   const int lanes = threadIdx.x & 3;
   for (int i0 = 0; i0 < slots; i0 += kThreads / 4) {
@@ -511,12 +512,14 @@ __device__ __forceinline__ void Prune(LongShared& s, int k, int slots, int prese
   __syncthreads();
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 4)
+// Threads: 256 (four CTAs an SM hide one another's barriers), or 512 for the
+// few rows that clusters share, whose time is that of one chunk after another.
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads)
     logprobs_long_kernel(const LogprobArgs a, int cluster) {
   using R = Row<T>;
   constexpr int kE = R::kN;
-  __shared__ LongShared s;
+  __shared__ LongShared<kThreads> s;
   pdl_trigger();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -843,13 +846,16 @@ void LaunchLogprobs(const LogprobArgs& a, cudaStream_t stream) {
   // 13.7 us with eight.
   constexpr int kVector = Row<T>::kN;
   int cluster = 1;
-  while (cluster < 8 && a.vocab >= cluster * 2 * kThreads * kVector) {
-    const bool long_parts = a.vocab >= cluster * 2 * 4 * kThreads * kVectors * kVector;
+  while (cluster < 8 && a.vocab >= cluster * 2 * 256 * kVector) {
+    const bool long_parts = a.vocab >= cluster * 2 * 4 * 256 * kVectors * kVector;
     if (items * cluster * 2 > (long_parts ? 4 : 2) * SmCount()) break;
     cluster *= 2;
   }
-  LaunchEx(logprobs_long_kernel<T>, dim3(static_cast<unsigned>(items * cluster)), dim3(kThreads), 0,
-           stream, what, static_cast<unsigned>(cluster), a, cluster);
+  // Large CTAs where all fit at once and have chunks enough.
+  const bool large = items * cluster <= SmCount() && a.vocab >= cluster * 2 * 256 * kVectors * kVector;
+  LaunchEx(large ? logprobs_long_kernel<T, 512> : logprobs_long_kernel<T, 256>,
+           dim3(static_cast<unsigned>(items * cluster)), dim3(large ? 512 : 256), 0, stream, what,
+           static_cast<unsigned>(cluster), a, cluster);
 }
 
 }  // namespace
