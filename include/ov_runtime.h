@@ -82,7 +82,8 @@ int ov_graph_destroy(ov_graph_t graph);
 enum {
   OV_DEVICE_WAIT_TIMEOUT = 1, /* a bounded wait ran out (no kernel of this library traps) */
   OV_DEVICE_BAD_ARGUMENT = 2  /* an index outside its range was skipped (a RoPE position,
-                                 an attention work item's sequence) */
+                                 an attention work item's sequence, a page or row bounds of
+                                 the 8-bit cache, a target token) */
 };
 
 /* Device-side error word written by kernels (bits above).  Reads and
