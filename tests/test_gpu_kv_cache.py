@@ -407,6 +407,71 @@ def test_a_nan_page_reaches_its_own_sequence_and_head_only(n):
         assert got[n:, 2 * D:].isnan().all()
 
 
+@pytest.mark.parametrize("heads", [17, 48, 200])
+def test_many_query_heads_of_one_key_head(heads):
+    """A single token's heads fill, or pass, a tile of rows."""
+    g = torch.Generator().manual_seed(heads)
+    lengths = [0, 1, 130, 300]
+    check_attention(filled(4, 32, 1, lengths, g), [1, 1, 2, 1], lengths, heads, True, g)
+
+
+@pytest.mark.parametrize("n", [1, 12, 40])
+def test_no_tokens_at_all(n):
+    g = torch.Generator().manual_seed(n)
+    gpu = GpuCache(filled(3, 16, 2, [0, 0, 0], g))
+    q = torch.randn(3 * n, 4 * D, generator=g).half().cuda()
+    out = torch.full_like(q, 5.0)
+    gpu.attend(q, [n] * 3, [0] * 3, 4, False, 0.1, out, gpu.workspace(3 * n, n, 0, 4))
+    torch.cuda.synchronize()
+    assert (out == 0).all()
+
+
+@pytest.mark.parametrize("n,heads,length,page", [(1, 2, 1_300_001, 16), (40, 1, 200_003, 64)])
+def test_a_very_long_history(n, heads, length, page):
+    """Against float64 on the GPU, in pieces."""
+    pages = -(-length // page)
+    g = torch.Generator(device="cuda").manual_seed(n)
+    table = torch.randperm(pages, generator=g, device="cuda").to(torch.int32)
+    codes = [torch.randint(-127, 128, (pages, 1, page, D), generator=g, device="cuda",
+                           dtype=torch.int8) for _ in range(2)]
+    scales = [torch.rand(pages, 1, generator=g, device="cuda") * 0.02 + 0.005 for _ in range(2)]
+    gpu = GpuCache(Cache(1, page, 1, torch.zeros(1, 1)))
+    gpu.codes, gpu.scales, gpu.table = codes, scales, table
+    d = gpu.desc
+    d.keys, d.values = codes[0].data_ptr(), codes[1].data_ptr()
+    d.key_scales, d.value_scales = scales[0].data_ptr(), scales[1].data_ptr()
+    d.page_table, d.pages, d.max_pages = table.data_ptr(), pages, pages
+    q = torch.randn(n, heads * D, generator=g, device="cuda").half()
+    out = torch.zeros_like(q)
+    gpu.attend(q, [n], [length], heads, True, D ** -0.5, out, gpu.workspace(n, n, length, heads))
+    torch.cuda.synchronize()
+    qd = q.double().view(n * heads, D)
+    row = torch.arange(n * heads, device="cuda") // heads
+    top = torch.full((n * heads, 1), -torch.inf, dtype=torch.float64, device="cuda")
+    total, acc, square = (torch.zeros(n * heads, w, dtype=torch.float64, device="cuda") for w in (1, D, D))
+    for p0 in range(0, pages, 20_000 * 16 // page):
+        at = table[p0:p0 + 20_000 * 16 // page].long()
+        k, v = ((codes[w][at, 0].double() * scales[w][at].double()[..., None]).flatten(0, 1)
+                for w in range(2))
+        pos = p0 * page + torch.arange(k.shape[0], device="cuda")
+        z = (qd @ k.T * D ** -0.5).masked_fill(pos > length - n + row[:, None], -torch.inf)
+        z = z.masked_fill(pos >= length, -torch.inf)
+        grown = torch.maximum(top, z.amax(-1, keepdim=True))
+        old, p = torch.exp(top - grown), torch.exp(z - grown)
+        total, acc = total * old + p.sum(-1, keepdim=True), acc * old + p @ v
+        square = square * old.square() + p.square() @ v.square()
+        top = grown
+    want = (acc / total).view(n, heads * D)
+    # The roundings of the probabilities to half, each within 2^-11 of its
+    # value, hence of a deviation of at most 2^-11 / sqrt(3) of it, are
+    # independent: their sum with the values deviates by that times the root of
+    # sum (p v)^2.  Seven deviations (2.6e-12 for a value, of 5,120), the
+    # output's own rounding, and as much again for float32 sums.
+    bound = (7 * 2.0 ** -11 / 3 ** 0.5 * square.sqrt() / total).view(n, heads * D)
+    bound = bound + want.abs() * 2.0 ** -10 + 2.0 ** -24
+    assert ((out.double() - want).abs() <= bound).all()
+
+
 @pytest.mark.parametrize("seqs,heads,kv", [(33, 4, 2), (64, 8, 8), (300, 2, 1), (1000, 1, 1)])
 @pytest.mark.parametrize("n", [1, 9])
 def test_many_sequences(seqs, heads, kv, n):

@@ -54,9 +54,9 @@ def check(x, codebooks, vocab, targets, k):
 
     The kernel's float32 error: the exponential's (2^-22, and its argument,
     rounded three times, by up to 1.5 * 2^-23 * |d| for a term e^d whose |d|
-    weighs |d| e^d <= 1/e) and a sum of at most 66 terms for a lane or
-    vocab / 512 + 100 for a thread, each off by 2^-24: a relative error of Z
-    below (vocab / 512 + 200) * 2^-24 + 2^-21.  A log probability adds the
+    weighs |d| e^d <= 1/e) and a sum of at most 66 terms for a lane or, in
+    sums of 4 or 8 values first, vocab / 1024 + 20 for a thread, each off by
+    2^-24: a relative error of Z below (vocab / 512 + 200) * 2^-24 + 2^-21.  A log probability adds the
     roundings of x - m, log Z and their difference, 2^-22 of |x - m| + log Z;
     the entropy's sum of e^d d has Z's relative error with |d| up to about
     its own size on top."""
@@ -92,7 +92,7 @@ def some_targets(x, codebooks, vocab, g):
 @pytest.mark.parametrize("rows,codebooks,vocab,k", [
     (1, 1, 1, 1), (3, 2, 2, 0), (5, 1, 31, 31), (9, 3, 33, 32), (7, 8, 1025, 5), (20, 1, 1056, 20),
     (4, 8, 1057, 32), (3, 2, 2112, 1), (2, 1, 2113, 32), (6, 3, 4099, 8), (2, 1, 8193, 20),
-    (1, 2, 16385, 32), (2, 1, 30000, 0), (1, 1, 151936, 20), (40, 1, 20011, 5)])
+    (1, 2, 16385, 32), (1, 1, 1 << 20, 32), (2, 1, 30000, 0), (1, 1, 151936, 20), (40, 1, 20011, 5)])
 def test_random_rows(rows, codebooks, vocab, k, half):
     """Rows at odd offsets; few rows of a long vocabulary share clusters."""
     g = torch.Generator().manual_seed(rows * vocab)
