@@ -1070,6 +1070,68 @@ __device__ __forceinline__ void IssueSingle(const TileIssue& mma, const AttnBars
   }
 }
 
+// Joins `parts` parts of a CTA's `here` rows, by 256 threads. Each L2 latency
+// costs about 1 us here, so a thread has two pieces (16 columns of a row) of two
+// parts in flight: 375 rows over 705 tokens took 18.2 us with one piece and four
+// parts, 16.3 with two and two, 18.3 with four and one (128 registers a thread
+// are all the compiler may use).
+template <typename OutRow>
+__device__ __forceinline__ void JoinTile(const TileArgs& args, const float* first, int parts, int here,
+                                         const OutRow& out_row) {
+  constexpr int kItems = 2;
+  const int stats_at = args.tile_rows * kCacheHeadDim;
+  for (int i0 = threadIdx.x; i0 < 8 * here; i0 += 256 * kItems) {
+    float top[kItems], sum[kItems], o[kItems][16];
+    int row[kItems], d16[kItems];
+#pragma unroll
+    for (int n = 0; n < kItems; ++n) {
+      const int i = min(i0 + n * 256, 8 * here - 1);  // behind the last: its sums again
+      d16[n] = i / here;
+      row[n] = i - d16[n] * here;
+      top[n] = -INFINITY;
+      sum[n] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) o[n][j] = 0.0f;
+    }
+#pragma unroll 2
+    for (int x = 0; x < parts; ++x) {
+      const float* p = first + x * TilePartFloats(args.tile_rows);
+      float2 ms[kItems];
+      float4 y[kItems][4];
+#pragma unroll
+      for (int n = 0; n < kItems; ++n) {
+        ms[n] = __ldcg(reinterpret_cast<const float2*>(p + stats_at + 2 * row[n]));
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          y[n][j] = __ldcg(reinterpret_cast<const float4*>(p) + (d16[n] * 4 + j) * args.tile_rows + row[n]);
+      }
+#pragma unroll
+      for (int n = 0; n < kItems; ++n) {
+        const float2 f = JoinFactors(&top[n], &sum[n], ms[n]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          o[n][4 * j] = fmaf(y[n][j].x, f.y, o[n][4 * j] * f.x);
+          o[n][4 * j + 1] = fmaf(y[n][j].y, f.y, o[n][4 * j + 1] * f.x);
+          o[n][4 * j + 2] = fmaf(y[n][j].z, f.y, o[n][4 * j + 2] * f.x);
+          o[n][4 * j + 3] = fmaf(y[n][j].w, f.y, o[n][4 * j + 3] * f.x);
+        }
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < kItems; ++n) {
+      if (i0 + n * 256 >= 8 * here) continue;
+      const float inv = sum[n] == 0.0f ? 0.0f : 1.0f / sum[n];
+      uint4* dst = reinterpret_cast<uint4*>(out_row(row[n]) + d16[n] * 16);
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        dst[j] = make_uint4(pack_half2(o[n][8 * j] * inv, o[n][8 * j + 1] * inv),
+                            pack_half2(o[n][8 * j + 2] * inv, o[n][8 * j + 3] * inv),
+                            pack_half2(o[n][8 * j + 4] * inv, o[n][8 * j + 5] * inv),
+                            pack_half2(o[n][8 * j + 6] * inv, o[n][8 * j + 7] * inv));
+    }
+  }
+}
+
 __global__ void __launch_bounds__(kTileThreads, 1)
     cache_attention_tile_kernel(const __grid_constant__ CUtensorMap map_k,
                                 const __grid_constant__ CUtensorMap map_v, const TileArgs args) {
@@ -1229,24 +1291,25 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     tmem_dealloc(tmem, 512);
   } else if (warp < kConvertWarp) {
     registers_grow<184>();
-    // Query rows into the swizzled tiles, 16 lanes a row, all loads in flight.
+    // Query rows into the swizzled tiles, 16 lanes a row, a tile's loads in flight.
     const int piece = tid & 15;
-    uint4 rows_in[16];
+    for (int tile = 0; tile < (pair ? 2 : 1); ++tile) {
+      uint4 rows_in[8];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int row = row0 + i * 16 + (tid >> 4), token = a.group(row);
-      rows_in[i] = make_uint4(0, 0, 0, 0);
-      if (row - row0 < here)
-        rows_in[i] = *reinterpret_cast<const uint4*>(
-            a.q + static_cast<int64_t>(span.first + token) * a.ld_q +
-            (kv_head * a.group.d + row - token * a.group.d) * kCacheHeadDim + piece * 8);
-    }
+      for (int i = 0; i < 8; ++i) {
+        const int row = row0 + tile * 128 + i * 16 + (tid >> 4), token = a.group(row);
+        rows_in[i] = make_uint4(0, 0, 0, 0);
+        if (row - row0 < here)
+          rows_in[i] = *reinterpret_cast<const uint4*>(
+              a.q + static_cast<int64_t>(span.first + token) * a.ld_q +
+              (kv_head * a.group.d + row - token * a.group.d) * kCacheHeadDim + piece * 8);
+      }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int r = i * 16 + (tid >> 4);
-      if (pair || i < 8)
-        *reinterpret_cast<uint4*>(q_s + (r >> 7) * kTile + (piece >> 3) * kHalfTile + (r & 127) * 128 +
+      for (int i = 0; i < 8; ++i) {
+        const int r = i * 16 + (tid >> 4);
+        *reinterpret_cast<uint4*>(q_s + tile * kTile + (piece >> 3) * kHalfTile + r * 128 +
                                   (((piece & 7) ^ (r & 7)) << 4)) = rows_in[i];
+      }
     }
     fence_proxy_async_smem();
     mbar_arrive(&s.q_full);
@@ -1466,36 +1529,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     named_barrier(1, 256);
     if (!s.last) return;
     const float* base_part = args.parts + item * args.splits * TilePartFloats(args.tile_rows);
-    for (int i = tid; i < 8 * here; i += 256) {
-      const int d16 = i / here, row = i - d16 * here;  // 16 columns of a row
-      float top = -INFINITY, sum = 0.0f;
-      float o[16] = {};
-#pragma unroll 4
-      for (int x = 0; x < parts; ++x) {
-        const float* p = base_part + x * TilePartFloats(args.tile_rows);
-        const float2 ms = __ldcg(reinterpret_cast<const float2*>(p + stats_at + 2 * row));
-        float4 y[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          y[j] = __ldcg(reinterpret_cast<const float4*>(p) + (d16 * 4 + j) * args.tile_rows + row);
-        const float2 f = JoinFactors(&top, &sum, ms);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          o[4 * j] = fmaf(y[j].x, f.y, o[4 * j] * f.x);
-          o[4 * j + 1] = fmaf(y[j].y, f.y, o[4 * j + 1] * f.x);
-          o[4 * j + 2] = fmaf(y[j].z, f.y, o[4 * j + 2] * f.x);
-          o[4 * j + 3] = fmaf(y[j].w, f.y, o[4 * j + 3] * f.x);
-        }
-      }
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      uint4* dst = reinterpret_cast<uint4*>(out_row(row) + d16 * 16);
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        dst[j] = make_uint4(pack_half2(o[8 * j] * inv, o[8 * j + 1] * inv),
-                            pack_half2(o[8 * j + 2] * inv, o[8 * j + 3] * inv),
-                            pack_half2(o[8 * j + 4] * inv, o[8 * j + 5] * inv),
-                            pack_half2(o[8 * j + 6] * inv, o[8 * j + 7] * inv));
-    }
+    JoinTile(args, base_part, parts, here, out_row);
   }
 }
 
