@@ -169,6 +169,13 @@ __device__ __forceinline__ void cp_async_4(void* dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src)
                : "memory");
 }
+// 16 bytes, or zeros where `there` is false (`src` is not read then).
+__device__ __forceinline__ void cp_async_16(void* dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src),
+               "r"(there ? 16 : 0)
+               : "memory");
+}
+
 // Arrives on `bar` when this thread's cp.asyncs so far have landed.
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar))
@@ -368,7 +375,7 @@ __global__ void __launch_bounds__(kStreamThreads + 128, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0);
   const int g = lane >> 2, c = lane & 3;
   // The rings of this warp, or (producers) of the one that this lane serves.
   const bool producer = warp >= kStreamWarps;
@@ -879,20 +886,28 @@ __global__ void __launch_bounds__(kStreamThreads + 128, 1)
 //           share every K and V tile;
 //   single  up to 128 rows: both warpgroups take the same tile, one the even
 //           and one the odd key tiles, and join at the end.
-// Bound per key tile by the MMAs and the softmax's exponentials as in
-// ov_attention_varlen: 4,800 cycles for 128 keys and 256 rows (a warpgroup's
-// softmax 2,500, its P V and next S 2,250, the two groups in turn), of which
-// the conversion of K and V, 1,200 cycles each, takes none of its own.
-// Measured on one B200: 16 causal sequences of up to 2,175 rows, 16 heads over
-// 8: 238 us, 520 TFLOP/s of what is seen; 375 rows over 705 tokens: 17.8 us,
-// where a CTA sees 2 key tiles and what comes before and after them counts
-// (first S 3.8 us after the start, parts written and joined in 5 us).
+// A softmax step takes 64 keys of a tile and S has two buffers for each
+// warpgroup, so that the S of the next 64 keys is there when it starts: with
+// one S of 128 keys the softmax and the products of a row tile took turns
+// (215 us for the case below, 197 with the two buffers).  The products are
+// issued by the elected thread of a converged warp: from a divergent branch
+// each instruction cost about 100 cycles, of 64 that the tensor core needs
+// (324 us with these 48 products a key tile, 240 with 32 of 128 keys).
 //
-// Registers: 512 threads start with 128 each; the softmax warpgroups, which
-// hold a row's 128 scores, take 184 and the other two keep 72.  With 128 for
-// all, scores read from tensor memory twice, a step took 7,100 cycles.
+// Bound by the softmax warps' latencies: 64 keys of both warpgroups take 2,200
+// cycles (waits 300, scores read and their maxima 500, exponentials and the
+// probabilities' way back 1,300; the MMAs take 1,280 beside that, K's and V's
+// conversion 1,600 a tile), and by what comes before and after a CTA's key
+// tiles, 7,400 and 3,100 cycles.  Measured on one B200: 16 causal sequences of
+// up to 2,175 rows, 16 heads over 8: 197 us, 632 TFLOP/s of what is seen; 375
+// rows over 705 tokens: 15.5 us, where a CTA sees 2 key tiles.
+//
+// Registers: 512 threads start with 128 each; the softmax warpgroups take 152,
+// the other two keep 104.
 
 constexpr int kSlabs = kKeys / 16;  // 16-key groups of a key tile: one page each at least
+constexpr int kUnitKeys = 64;       // keys of one softmax step: half a key tile
+constexpr int kUnitSlabs = kUnitKeys / 16;
 constexpr int kScaleSlots = 8;
 constexpr int kMinKeyTiles = 2;  // of a split; 2 to 4 measured alike (375 rows over 705 tokens
                                  // 18.0 to 17.2 us), 8 took 24.2 us for 19.6 over 2,048 tokens
@@ -908,7 +923,8 @@ struct alignas(16) SlabScale {
 };
 
 struct TileShared {
-  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2];
+  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t s_full[2][2], p_full[2][2];     // [group][buffer]
   uint64_t codes_full[2], codes_empty[2];  // of keys, of values
   uint64_t scale_full[kScaleSlots];
   uint32_t tmem;
@@ -945,8 +961,7 @@ __device__ __forceinline__ float Max16(const uint32_t* r) {
 }
 
 // 16 codes to 16 halves, in two 16-byte pieces.
-__device__ __forceinline__ void Convert16(const uint8_t* codes, uint8_t* low, uint8_t* high) {
-  const uint4 q = *reinterpret_cast<const uint4*>(codes);
+__device__ __forceinline__ void Convert16(const uint4& q, uint8_t* low, uint8_t* high) {
   const uint32_t x = q.x ^ 0x80808080u, y = q.y ^ 0x80808080u;
   const uint32_t z = q.z ^ 0x80808080u, w = q.w ^ 0x80808080u;
   *reinterpret_cast<uint4*>(low) =
@@ -967,15 +982,27 @@ __device__ __forceinline__ void ConvertTile(const uint8_t* codes, uint8_t* tile,
   const uint32_t first = box * kHalfTile, second = kHalfTile - first;
   const uint8_t* src_first = src + box * 64;
   const uint8_t* src_second = src + 64 - box * 64;
-#pragma unroll 2
+  uint4 q[8];
+#pragma unroll
   for (int i = 0; i < 4; ++i) {
-    Convert16(src_first + i * 32 * kCacheHeadDim, low + first + i * 32 * 128, high + first + i * 32 * 128);
-    Convert16(src_second + i * 32 * kCacheHeadDim, low + second + i * 32 * 128, high + second + i * 32 * 128);
+    q[2 * i] = *reinterpret_cast<const uint4*>(src_first + i * 32 * kCacheHeadDim);
+    q[2 * i + 1] = *reinterpret_cast<const uint4*>(src_second + i * 32 * kCacheHeadDim);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    Convert16(q[2 * i], low + first + i * 32 * 128, high + first + i * 32 * 128);
+    Convert16(q[2 * i + 1], low + second + i * 32 * 128, high + second + i * 32 * 128);
   }
 }
 
-// The products of one CTA, issued by one thread.  A step along the head
-// dimension or the keys only adds to a descriptor's address field.
+// One arrival for a warp, behind what all its lanes did.
+__device__ __forceinline__ void WarpArrive(uint64_t* bar) {
+  __syncwarp();
+  if (elect_one()) mbar_arrive(bar);
+}
+
+// The products of one CTA, issued by one thread of a converged warp.  A step
+// along the head dimension or the keys only adds to a descriptor's address field.
 struct TileIssue {
   uint32_t tmem;
   uint64_t q, k, v;  // descriptors of row tile 0 and of stage 0
@@ -986,86 +1013,116 @@ struct TileIssue {
         q(smem_desc_sw128(smem_u32(q_s), 16, 1024)),
         k(smem_desc_sw128(smem_u32(k_s), 16, 1024)),
         v(smem_desc_sw128(smem_u32(v_s), kHalfTile, 1024)) {}
-  // S of group g = Q of row tile `tile` x K of `stage`.
-  __device__ __forceinline__ void Scores(int g, int tile, int stage) const {
-    constexpr uint32_t idesc = idesc_f16_f32(kQ, kKeys, 0);
+  // S of group g, buffer `half` = Q of row tile `tile` x that half of K of `stage`.
+  __device__ __forceinline__ void Scores(int g, int tile, int stage, int half) const {
+    constexpr uint32_t idesc = idesc_f16_f32(kQ, kUnitKeys, 0);
     const uint64_t qd = q + static_cast<uint32_t>(tile) * (kTile >> 4);
-    const uint64_t kd = k + static_cast<uint32_t>(stage) * (kTile >> 4);
+    const uint64_t kd = k + static_cast<uint32_t>(stage) * (kTile >> 4) +
+                        static_cast<uint32_t>(half) * (kUnitKeys * 128 >> 4);
+    const uint32_t d = tmem + static_cast<uint32_t>(g * 256 + half * kUnitKeys);
+    if (!elect_one()) return;
 #pragma unroll
     for (int kk = 0; kk < kD / 16; ++kk) {
       const uint32_t off = ((kk >> 2) * kHalfTile + (kk & 3) * 32) >> 4;
-      umma_f16_ss(tmem + static_cast<uint32_t>(g * 256), qd + off, kd + off, idesc, kk > 0 ? 1u : 0u);
+      umma_f16_ss(d, qd + off, kd + off, idesc, kk > 0 ? 1u : 0u);
     }
   }
-  // O of group g (+)= its P x V of `stage`.
-  __device__ __forceinline__ void Values(int g, int stage, bool add) const {
+  // O of group g (+)= P of buffer `half` x that half of V of `stage`.
+  __device__ __forceinline__ void Values(int g, int stage, int half, bool add) const {
     constexpr uint32_t idesc = idesc_f16_f32(kQ, kD, 1);
-    const uint64_t vd = v + static_cast<uint32_t>(stage) * (kTile >> 4);
-    const uint32_t p = tmem + static_cast<uint32_t>(g * 256);
+    const uint64_t vd = v + static_cast<uint32_t>(stage) * (kTile >> 4) +
+                        static_cast<uint32_t>(half) * (kUnitKeys * 128 >> 4);
+    const uint32_t o = tmem + static_cast<uint32_t>(g * 256 + 128);
+    const uint32_t p = tmem + static_cast<uint32_t>(g * 256 + half * kUnitKeys);
+    if (!elect_one()) return;
 #pragma unroll
-    for (int kk = 0; kk < kKeys / 16; ++kk)
-      umma_f16_ts(p + 128, p + static_cast<uint32_t>(kk * 8), vd + ((kk * 16 * 128) >> 4), idesc,
+    for (int kk = 0; kk < kUnitKeys / 16; ++kk)
+      umma_f16_ts(o, p + static_cast<uint32_t>(kk * 8), vd + ((kk * 16 * 128) >> 4), idesc,
                   add || kk > 0 ? 1u : 0u);
   }
 };
 
-// Two row tiles share every key tile: while the softmax works on one group's
-// S the tensor core runs the other's products.
-__device__ __forceinline__ void IssuePairs(const TileIssue& mma, const AttnBars& bars, int nt,
-                                           uint32_t* err) {
-  if (!mbar_wait(bars.q_full, 0, err) || !mbar_wait(&bars.k_full[0], 0, err)) return;
+__device__ __forceinline__ void Commit(uint64_t* bar) {
+  if (elect_one()) umma_commit(bar);
+}
+
+// A wait of the whole warp, converged behind it, with one outcome for all.
+__device__ __forceinline__ bool WarpWait(uint64_t* bar, uint32_t parity, uint32_t* err) {
+  return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, err));
+}
+
+// Phases of the barriers: s_full[g][b] completes once for the first S of the
+// buffer, then once for each of its P V (and the S after it, where there is
+// one); p_full[g][b] once for each P.  So S of unit u is there after phase
+// u / 2, and P V of unit u is done after phase u / 2 + 1.
+
+// Two row tiles share every key tile.  units0, units1: 64-key units of which the
+// groups' rows see something; one of the groups reaches the last key tile.
+__device__ __forceinline__ void IssuePairs(const TileIssue& mma, TileShared& s, int nt, int units0,
+                                           int units1, uint32_t* err) {
+  if (!WarpWait(&s.q_full, 0, err) || !WarpWait(&s.k_full[0], 0, err)) return;
   tc_fence_after_sync();
 #pragma unroll 1
-  for (int g = 0; g < 2; ++g) {
-    mma.Scores(g, g, 0);
-    umma_commit(&bars.s_full[g]);
+  for (int i = 0; i < 4; ++i) {
+    const int half = i >> 1, g = i & 1;
+    if (half >= (g == 0 ? units0 : units1)) continue;
+    mma.Scores(g, g, 0, half);
+    Commit(&s.s_full[g][half]);
   }
-  umma_commit(&bars.k_empty[0]);
+  Commit(&s.k_empty[0]);
 #pragma unroll 1
   for (int t = 0; t < nt; ++t) {
     const int stage = t & 1, next = stage ^ 1;
+    bool k_ready = false;
+    if (!WarpWait(&s.v_full[stage], static_cast<uint32_t>(t >> 1) & 1u, err)) return;
 #pragma unroll 1
-    for (int g = 0; g < 2; ++g) {
-      if (!mbar_wait(&bars.p_full[g], static_cast<uint32_t>(t) & 1u, err) ||
-          (g == 0 && !mbar_wait(&bars.v_full[stage], static_cast<uint32_t>(t >> 1) & 1u, err)))
-        return;
+    for (int i = 0; i < 4; ++i) {
+      const int half = i >> 1, g = i & 1, u = 2 * t + half, units = g == 0 ? units0 : units1;
+      if (u >= units) continue;
+      if (!WarpWait(&s.p_full[g][half], static_cast<uint32_t>(t) & 1u, err)) return;
       tc_fence_after_sync();
-      mma.Values(g, stage, t > 0);
-      if (t + 1 == nt) {
-        umma_commit(&bars.o_done[g]);
-        continue;
+      mma.Values(g, stage, half, u > 0);
+      if (u + 2 < units) {
+        if (!k_ready && !WarpWait(&s.k_full[next], static_cast<uint32_t>((t + 1) >> 1) & 1u, err)) return;
+        k_ready = true;
+        tc_fence_after_sync();
+        mma.Scores(g, g, next, half);
       }
-      if (g == 0 && !mbar_wait(&bars.k_full[next], static_cast<uint32_t>((t + 1) >> 1) & 1u, err)) return;
-      tc_fence_after_sync();
-      mma.Scores(g, g, next);
-      umma_commit(&bars.s_full[g]);
+      Commit(&s.s_full[g][half]);
     }
-    umma_commit(&bars.v_empty[stage]);
-    if (t + 1 < nt) umma_commit(&bars.k_empty[next]);
+    Commit(&s.v_empty[stage]);
+    if (t + 1 < nt) Commit(&s.k_empty[next]);
   }
 }
 
-// One row tile: key tile t belongs to group t & 1.
-__device__ __forceinline__ void IssueSingle(const TileIssue& mma, const AttnBars& bars, int nt,
-                                            uint32_t* err) {
-  if (!mbar_wait(bars.q_full, 0, err)) return;
-  for (int t = -2; t < nt; ++t) {
-    const int g = t & 1;
-    if (t >= 0) {
+// One row tile: key tile t belongs to group t & 1, in stage t & 1.  (Products in
+// the order in which their operands arrive, polled, were alike here and 5 % slower
+// for pairs; a second issuing warp was 3 % slower.)
+__device__ __forceinline__ void IssueSingle(const TileIssue& mma, TileShared& s, int nt, int units0,
+                                            int units1, uint32_t* err) {
+  if (!WarpWait(&s.q_full, 0, err)) return;
+  for (int t = -2; t < nt; t += 2) {  // tiles t and t + 1; before the first, only their S
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i) {
+      // A tile's two units before the other group's: keys of tile t + 3 are
+      // converted behind the values of t + 2, which wait for those of tile t.
+      const int half = i & 1, g = i >> 1;
+      const int u = t + half, units = g == 0 ? units0 : units1;
       const uint32_t phase = static_cast<uint32_t>(t >> 1) & 1u;
-      if (!mbar_wait(&bars.p_full[g], phase, err) || !mbar_wait(&bars.v_full[g], phase, err)) return;
-      tc_fence_after_sync();
-      mma.Values(g, g, t > 1);
-      umma_commit(&bars.v_empty[g]);
-    }
-    if (t + 2 < nt) {
-      if (!mbar_wait(&bars.k_full[g], static_cast<uint32_t>((t + 2) >> 1) & 1u, err)) return;
-      tc_fence_after_sync();
-      mma.Scores(g, 0, g);
-      umma_commit(&bars.s_full[g]);
-      umma_commit(&bars.k_empty[g]);
-    } else if (t >= 0) {
-      umma_commit(&bars.o_done[g]);
+      if (t >= 0 && u < units) {
+        if (!WarpWait(&s.p_full[g][half], phase, err)) return;
+        if (half == 0 && !WarpWait(&s.v_full[g], phase, err)) return;
+        tc_fence_after_sync();
+        mma.Values(g, g, half, u > 0);
+        if (half == 1 || u + 1 == units) Commit(&s.v_empty[g]);
+      }
+      if (u + 2 < units) {
+        if (half == 0 && !WarpWait(&s.k_full[g], phase ^ 1u, err)) return;
+        tc_fence_after_sync();
+        mma.Scores(g, 0, g, half);
+        if (half == 1 || u + 3 == units) Commit(&s.k_empty[g]);
+      }
+      if (u + 2 < units || (t >= 0 && u < units)) Commit(&s.s_full[g][half]);
     }
   }
 }
@@ -1073,8 +1130,7 @@ __device__ __forceinline__ void IssueSingle(const TileIssue& mma, const AttnBars
 // Joins `parts` parts of a CTA's `here` rows, by 256 threads. Each L2 latency
 // costs about 1 us here, so a thread has two pieces (16 columns of a row) of two
 // parts in flight: 375 rows over 705 tokens took 18.2 us with one piece and four
-// parts, 16.3 with two and two, 18.3 with four and one (128 registers a thread
-// are all the compiler may use).
+// parts, 16.3 with two and two, 18.3 with four and one.
 template <typename OutRow>
 __device__ __forceinline__ void JoinTile(const TileArgs& args, const float* first, int parts, int here,
                                          const OutRow& out_row) {
@@ -1140,26 +1196,39 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   pdl_trigger();
   pdl_wait();
   // Heads first: CTAs that run together read whole rows of q and whole pages.
-  // The last row tiles of a causal sequence see most: they start first.
-  const int kv_head = static_cast<int>(blockIdx.x) % cache.kv_heads, seq = blockIdx.y;
-  const int part_of_rows = static_cast<int>(blockIdx.x) / cache.kv_heads;
-  const int tile = args.tiles - 1 - part_of_rows / args.splits;
-  const int split = part_of_rows % args.splits;
+  // The last row tiles of causal sequences see most: they start first, those
+  // of all sequences before the next.
+  int at_grid = static_cast<int>(blockIdx.x);
+  const int kv_head = at_grid % cache.kv_heads;
+  at_grid /= cache.kv_heads;
+  const int split = at_grid % args.splits;
+  at_grid /= args.splits;
+  const int seq = at_grid % cache.num_seqs;
+  const int tile = args.tiles - 1 - at_grid / cache.num_seqs;
+  const int announced = a.lengths[seq];
   const RowSpan span = SequenceRows(a.cu_rows, seq, a.rows, a.max_rows, a.err);
   const int rows = span.count * a.group.d;  // at most 2^31 (host check)
   const int row0 = tile * args.tile_rows;
   if (row0 >= rows) return;  // uniform over the CTA, before any barrier
-  const int length = CheckLength(a, a.lengths[seq]);
+  const int length = CheckLength(a, announced);
   const bool pair = rows - row0 > kQ && args.tile_rows > kQ;
   const int here = min(rows - row0, args.tile_rows);
-  const int last_token = a.group(row0 + here - 1);
-  const int reach = a.causal ? max(0, length - span.count + last_token + 1) : length;
+  const int before = length - span.count;  // tokens that row token 0 has before it
+  // Tokens that some row up to (and with) row0 + n sees.
+  auto reach_of = [&](int n) { return a.causal ? max(0, before + a.group(row0 + n) + 1) : length; };
+  const int reach = reach_of(here - 1);
   const int all_tiles = (reach + kKeys - 1) / kKeys;
   const int per = max(1, (all_tiles + args.splits - 1) / args.splits);
   const int parts = max(1, (all_tiles + per - 1) / per);
   if (split >= parts) return;
   const int t0 = split * per;
   const int nt = min(all_tiles, t0 + per) - t0;
+  // 64-key units of the groups: of a pair's first tile up to what its rows see,
+  // else the even and the odd key tiles'.
+  auto units_of = [&](int r) { return max(0, min(2 * nt, (r - t0 * kKeys + kUnitKeys - 1) / kUnitKeys)); };
+  const int all_units = units_of(reach);
+  const int units0 = pair ? units_of(reach_of(kQ - 1)) : (nt + 1) / 2 * 2 - ((nt & 1) != 0 ? all_units & 1 : 0);
+  const int units1 = pair ? all_units : nt / 2 * 2 - ((nt & 1) == 0 ? all_units & 1 : 0);
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -1169,29 +1238,33 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint8_t* v_s = k_s + 2 * kTile;    // [2 stages] x 32 KB
   uint8_t* code_s = v_s + 2 * kTile; // keys, values: 16 KB each
   TileShared& s = *reinterpret_cast<TileShared*>(code_s + 2 * kCodeTile);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  AttnBars bars;
-  bars.q_full = &s.q_full;
-  bars.k_full = s.k_full;
-  bars.k_empty = s.k_empty;
-  bars.v_full = s.v_full;
-  bars.v_empty = s.v_empty;
-  bars.s_full = s.s_full;
-  bars.p_full = s.p_full;
-  bars.o_done = s.o_done;
-  bars.pv_done = nullptr;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0);
+  // Query rows into the swizzled tiles, 16 lanes a row, by the softmax warps:
+  // on their way while the CTA sets itself up.
+  const int piece = tid & 15;
+  if (tid < kConvertWarp * 32) {
+    for (int r = tid >> 4; r < (pair ? 2 * kQ : kQ); r += 16) {
+      const int row = row0 + min(r, here - 1), token = a.group(row);
+      cp_async_16(q_s + (r >> 7) * kTile + (piece >> 3) * kHalfTile + (r & 127) * 128 +
+                      (((piece & 7) ^ (r & 7)) << 4),
+                  a.q + static_cast<int64_t>(span.first + token) * a.ld_q +
+                      (kv_head * a.group.d + row - token * a.group.d) * kCacheHeadDim + piece * 8,
+                  r < here);
+    }
+  }
   if (tid == 0) {
-    mbar_init(&s.q_full, 256);
+    mbar_init(&s.q_full, 8);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&s.k_full[i], 128);
-      mbar_init(&s.v_full[i], 128);
+      mbar_init(&s.k_full[i], 4);
+      mbar_init(&s.v_full[i], 4);
       mbar_init(&s.codes_full[i], kSlabs);
-      mbar_init(&s.codes_empty[i], 128);
+      mbar_init(&s.codes_empty[i], 4);
       mbar_init(&s.k_empty[i], 1);
       mbar_init(&s.v_empty[i], 1);
-      mbar_init(&s.s_full[i], 1);
-      mbar_init(&s.p_full[i], 128);
-      mbar_init(&s.o_done[i], 1);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&s.s_full[i][b], 1);
+        mbar_init(&s.p_full[i][b], 4);
+      }
     }
     for (int i = 0; i < kScaleSlots; ++i) mbar_init(&s.scale_full[i], kSlabs);
     fence_mbar_init();
@@ -1205,12 +1278,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  const uint32_t tmem = s.tmem;
+  const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, s.tmem, 0);
   const int64_t item = (static_cast<int64_t>(tile) * cache.num_seqs + seq) * cache.kv_heads + kv_head;
   float* part = parts > 1 ? args.parts + (item * args.splits + split) * TilePartFloats(args.tile_rows) : nullptr;
   const int stats_at = args.tile_rows * kCacheHeadDim;
 
-  if (warp >= kConvertWarp) registers_shrink<72>();
+  if (warp >= kConvertWarp) registers_shrink<104>();
   if (warp == kLoadWarp) {
     // Lane i < 8 looks after slab i of a key tile; the first slab of a box
     // loads it.  Codes wait for the converters, one key tile ahead of them.
@@ -1270,49 +1343,30 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       if (t >= 2) ok = ok && mbar_wait(&s.k_empty[stage], reuse, a.err);
       ConvertTile(code_s, k_s + stage * kTile, ctid);
       fence_proxy_async_smem();
-      mbar_arrive(&s.k_full[stage]);
-      mbar_arrive(&s.codes_empty[0]);
+      WarpArrive(&s.k_full[stage]);
+      WarpArrive(&s.codes_empty[0]);
       ok = ok && mbar_wait(&s.codes_full[1], static_cast<uint32_t>(t) & 1u, a.err);
       if (t >= 2) ok = ok && mbar_wait(&s.v_empty[stage], reuse, a.err);
       ConvertTile(code_s + kCodeTile, v_s + stage * kTile, ctid);
       fence_proxy_async_smem();
-      mbar_arrive(&s.v_full[stage]);
-      mbar_arrive(&s.codes_empty[1]);
+      WarpArrive(&s.v_full[stage]);
+      WarpArrive(&s.codes_empty[1]);
     }
   } else if (warp == kMmaWarp) {
-    if (lane == 0 && nt > 0) {
+    if (nt > 0) {
       const TileIssue mma(tmem, q_s, k_s, v_s);
-      if (pair) IssuePairs(mma, bars, nt, a.err);
-      else IssueSingle(mma, bars, nt, a.err);
+      if (pair) IssuePairs(mma, s, nt, units0, units1, a.err);
+      else IssueSingle(mma, s, nt, units0, units1, a.err);
     }
     __syncwarp();
     named_barrier(2, 256 + 32);  // O was read
     tc_fence_after_sync();
     tmem_dealloc(tmem, 512);
   } else if (warp < kConvertWarp) {
-    registers_grow<184>();
-    // Query rows into the swizzled tiles, 16 lanes a row, a tile's loads in flight.
-    const int piece = tid & 15;
-    for (int tile = 0; tile < (pair ? 2 : 1); ++tile) {
-      uint4 rows_in[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int row = row0 + tile * 128 + i * 16 + (tid >> 4), token = a.group(row);
-        rows_in[i] = make_uint4(0, 0, 0, 0);
-        if (row - row0 < here)
-          rows_in[i] = *reinterpret_cast<const uint4*>(
-              a.q + static_cast<int64_t>(span.first + token) * a.ld_q +
-              (kv_head * a.group.d + row - token * a.group.d) * kCacheHeadDim + piece * 8);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = i * 16 + (tid >> 4);
-        *reinterpret_cast<uint4*>(q_s + tile * kTile + (piece >> 3) * kHalfTile + r * 128 +
-                                  (((piece & 7) ^ (r & 7)) << 4)) = rows_in[i];
-      }
-    }
+    registers_grow<152>();
+    cp_async_wait_all();
     fence_proxy_async_smem();
-    mbar_arrive(&s.q_full);
+    WarpArrive(&s.q_full);
 
     const int g = warp >> 2;
     const int r = tid & 127;               // tensor-memory lane, row of the tile
@@ -1320,34 +1374,34 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem + static_cast<uint32_t>(g * 256) + lanes;
     const uint32_t o_addr = s_addr + 128;
-    const int before = length - span.count;  // tokens that row token 0 has before it
     const int seen = a.causal ? min(length, before + a.group(mine) + 1) : length;
     // The fewest tokens that a row of this tile sees.
     const int least = a.causal ? before + a.group(mine - r) + 1 : length;
-    const int step = pair ? 1 : 2, first = pair ? 0 : g;
+    const int units = g == 0 ? units0 : units1;
     float m = -INFINITY, l = 0.0f;
-    int use = 0;
     bool ok = true;
-    for (int t = first; t < nt; t += step, ++use) {
+    for (int u = 0; u < units; ++u) {
+      const int half = u & 1, t = pair ? u >> 1 : (u & ~1) + g;
+      const uint32_t p_addr = s_addr + static_cast<uint32_t>(half * kUnitKeys);
       ok = ok && mbar_wait(&s.scale_full[t % kScaleSlots],
                            static_cast<uint32_t>(t / kScaleSlots) & 1u, a.err);
-      const SlabScale* slab = s.scales[t % kScaleSlots];
-      ok = ok && mbar_wait(&s.s_full[g], static_cast<uint32_t>(use) & 1u, a.err);
+      const SlabScale* slab = s.scales[t % kScaleSlots] + half * kUnitSlabs;
+      ok = ok && mbar_wait(&s.s_full[g][half], static_cast<uint32_t>(u >> 1) & 1u, a.err);
       __syncwarp();
       tc_fence_after_sync();
-      const int token0 = (t0 + t) * kKeys;
+      const int token0 = (t0 + t) * kKeys + half * kUnitKeys;
       int bad = 0;
 #pragma unroll
-      for (int i = 0; i < kSlabs; ++i) bad |= slab[i].bad;
-      const bool partial = token0 + kKeys > least || bad != 0;
-      uint32_t x[4][32];
+      for (int i = 0; i < kUnitSlabs; ++i) bad |= slab[i].bad;
+      const bool partial = token0 + kUnitKeys > least || bad != 0;
+      uint32_t x[2][32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_addr + c * 32, x[c]);
+      for (int c = 0; c < 2; ++c) tmem_ld_32x32b_x32(p_addr + c * 32, x[c]);
       tmem_ld_wait();
       if (partial) {
         const int valid = seen - token0;
 #pragma unroll
-        for (int i = 0; i < kSlabs; ++i) {
+        for (int i = 0; i < kUnitSlabs; ++i) {
           const int slab_valid = slab[i].bad != 0 ? 0 : valid - i * 16;
 #pragma unroll
           for (int j = 0; j < 16; ++j)
@@ -1362,13 +1416,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       };
       float top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < kSlabs; ++i) {
+      for (int i = 0; i < kUnitSlabs; ++i) {
         const SlabScale k = scale_of(i);
         top = fmaxf(top, fmaf(Max16(&x[i >> 1][(i & 1) * 16]), k.factor, k.shift));
       }
       bool rescale = false;
       float alpha = 1.0f;
-      if (use == 0) {
+      if (u == 0) {
         m = top;
       } else {
         const bool grow = top > m + kRescaleThreshold;
@@ -1381,27 +1435,36 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const float base = m == -INFINITY ? 0.0f : m;
       float sum = 0.0f;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 2; ++c) {
         uint32_t packed[16];
+        float e[32];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const SlabScale k = scale_of(c * 2 + i);
           const float shift = k.shift - base;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) e[i * 16 + j] = fmaf(__uint_as_float(x[c][i * 16 + j]), k.factor, shift);
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) e[j] = ex2_approx(e[j]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
           float p0 = 0.0f, p1 = 0.0f;
 #pragma unroll
           for (int j = 0; j < 16; j += 2) {
-            const float e0 = ex2_approx(fmaf(__uint_as_float(x[c][i * 16 + j]), k.factor, shift));
-            const float e1 = ex2_approx(fmaf(__uint_as_float(x[c][i * 16 + j + 1]), k.factor, shift));
-            p0 += e0;
-            p1 += e1;
-            packed[i * 8 + j / 2] = pack_half2(e0, e1);
+            p0 += e[i * 16 + j];
+            p1 += e[i * 16 + j + 1];
+            packed[i * 8 + j / 2] = pack_half2(e[i * 16 + j], e[i * 16 + j + 1]);
           }
-          sum = fmaf(p0 + p1, k.inverse, sum);
+          sum = fmaf(p0 + p1, scale_of(c * 2 + i).inverse, sum);
         }
-        tmem_st_32x32b_x16(s_addr + c * 16, packed);
+        tmem_st_32x32b_x16(p_addr + c * 16, packed);
       }
-      if (rescale) {
+      if (rescale) {  // O so far: behind the P V of the unit before
         l *= alpha;
+        ok = ok && mbar_wait(&s.s_full[g][half ^ 1], static_cast<uint32_t>(((u - 1) >> 1) + 1) & 1u, a.err);
+        __syncwarp();
+        tc_fence_after_sync();
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t x[32];
@@ -1416,19 +1479,19 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       l += sum;
       tmem_st_wait();
       tc_fence_before_sync();
-      mbar_arrive(&s.p_full[g]);
+      WarpArrive(&s.p_full[g][half]);
     }
 
     // O of this warpgroup's tile.  In the single form the warpgroups have the
     // even and the odd key tiles' parts of one tile: each takes half of the
     // columns, the other's half comes through shared memory (every MMA is
     // done by then, so the rings are idle).  Columns here: [col0, col0 + 32 n).
-    if (pair && nt > 0) ok = ok && mbar_wait(&s.o_done[g], 0, a.err);
-    if (!pair && nt > 0) ok = ok && mbar_wait(&s.o_done[0], 0, a.err);
-    if (!pair && nt > 1) ok = ok && mbar_wait(&s.o_done[1], 0, a.err);
+    if (units > 0)
+      ok = ok && mbar_wait(&s.s_full[g][(units - 1) & 1], static_cast<uint32_t>(((units - 1) >> 1) + 1) & 1u, a.err);
+    if (!pair) named_barrier(1, 256);
     __syncwarp();
     tc_fence_after_sync();
-    const bool mine_any = nt > first, other_any = !pair && nt > 1 - first;
+    const bool mine_any = units > 0, other_any = !pair && (g == 0 ? units1 : units0) > 0;
     const int chunks = pair ? 4 : 2, col0 = pair ? 0 : g * 64;
     float4* exchange = reinterpret_cast<float4*>(k_s);  // [group][16 vectors][128 rows]
     float2* stats = reinterpret_cast<float2*>(v_s);     // [group][128 rows]
@@ -1699,6 +1762,8 @@ int ov_attention_kv_cache(const ov_kv_cache* cache, const uint16_t* q, size_t ld
         args.splits = 1;
       }
     }
+    const size_t grid = static_cast<size_t>(args.tiles) * args.splits * cache->kv_heads * cache->num_seqs;
+    OV_REQUIRE(grid <= INT32_MAX, "max_rows times the sequences and heads is above what one launch takes");
     const size_t box = std::min<size_t>(kKeys, cache->page_tokens);
     CUtensorMap map_k, map_v;
     EncodeCodesMap(&map_k, c.keys, cache, box, CU_TENSOR_MAP_SWIZZLE_NONE);
@@ -1706,8 +1771,7 @@ int ov_attention_kv_cache(const ov_kv_cache* cache, const uint16_t* q, size_t ld
     SetMaxDynamicSmem(reinterpret_cast<const void*>(cache_attention_tile_kernel),
                       static_cast<int>(kTileSmem));
     Launch(cache_attention_tile_kernel,
-           dim3(static_cast<unsigned>(args.tiles) * static_cast<unsigned>(args.splits * c.kv_heads),
-                static_cast<unsigned>(c.num_seqs)),
+           dim3(static_cast<unsigned>(grid)),
            dim3(kTileThreads), kTileSmem, AsStream(stream), "cache attention kernel launch", map_k,
            map_v, args);
   });

@@ -415,6 +415,26 @@ def test_many_query_heads_of_one_key_head(heads):
     check_attention(filled(4, 32, 1, lengths, g), [1, 1, 2, 1], lengths, heads, True, g)
 
 
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("heads,kv", [(8, 8), (16, 8), (24, 8)])
+def test_lengths_around_the_kernels_key_steps_in_pairs_of_row_tiles(heads, kv, causal):
+    """So many sequences that a CTA takes 256 rows, of which the first 128 may
+    see up to 128 tokens less than the last."""
+    g = torch.Generator().manual_seed(heads + causal)
+    lengths = [n + d for n in (64, 128, 192, 256, 320, 640, 1152) for d in (-1, 0, 1)]
+    counts = [min(n, 129 + 17 * i) for i, n in enumerate(lengths)]
+    counts[:3] = [129, 256, 257]  # more rows than tokens: the first see none
+    check_attention(filled(len(lengths), 64, kv, lengths, g), counts, lengths, heads, causal, g)
+
+
+@pytest.mark.parametrize("workspace", [True, False])
+@pytest.mark.parametrize("length", [1, 63, 64, 65, 127, 128, 129, 193, 256, 257, 384, 449, 511, 640, 1025, 1151])
+def test_lengths_around_the_kernels_key_steps_in_single_tiles(length, workspace):
+    g = torch.Generator().manual_seed(length)
+    check_attention(filled(1, 16, 2, [length], g), [40], [length], 4, True, g, workspace)
+    check_attention(filled(1, 128, 2, [length], g), [100], [length], 2, False, g, workspace)
+
+
 @pytest.mark.parametrize("n", [1, 12, 40])
 def test_no_tokens_at_all(n):
     g = torch.Generator().manual_seed(n)
