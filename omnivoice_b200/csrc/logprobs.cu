@@ -12,10 +12,11 @@
 //
 // Measured on one B200: the audio head's 500 rows of 8 x 1,025 float32 values
 // (16.6 MB) 8.0 us; 512 half rows of 151,936 values (156 MB) with 20
-// alternatives 56 us, 2.8 TB/s: not the reading but about 15 instructions for
-// a value bound it (7.6 for the sums and the rank, the rest for alternatives
-// and what a chunk costs); one float32 row of that length 13.9 us, its
-// clusters' barriers and joins included.
+// alternatives 52 us, 3.0 TB/s: not the reading but about 13 instructions for
+// a value bound it (6 for the sums and the rank, the rest for alternatives and
+// what a chunk costs; with the sums' operations one by one instead of in pairs,
+// 56 us); one float32 row of that length 12.6 us, its clusters' barriers and
+// joins included.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -169,6 +170,14 @@ struct Row<float> {
   static __device__ __forceinline__ float Exponent(float x, float scaled) {
     return (x - scaled) * kLog2E;
   }
+  // Those of values i and i + 1; finite, so that a closed token's 0 * t is 0.
+  static __device__ __forceinline__ float2 Exponents(const uint4& q, int i, float scaled) {
+    return Finite(mul2(add2(make_float2(At(q, i), At(q, i + 1)), make_float2(-scaled, -scaled)),
+                       make_float2(kLog2E, kLog2E)));
+  }
+  static __device__ __forceinline__ float2 Finite(float2 t) {
+    return make_float2(fmaxf(t.x, -16384.0f), fmaxf(t.y, -16384.0f));
+  }
   // log p of a value, with log_z = log Z.
   static __device__ __forceinline__ float LogProb(float x, float m, float log_z) {
     return (x - m) - log_z;
@@ -224,6 +233,11 @@ struct Row<__half> {
   static __device__ __forceinline__ float Scaled(float m) { return __fmul_rn(m, kLog2E); }
   static __device__ __forceinline__ float Exponent(float x, float scaled) {
     return fmaf(x, kLog2E, -scaled);
+  }
+  static __device__ __forceinline__ float2 Exponents(const uint4& q, int i, float scaled) {
+    const uint32_t w = i < 2 ? q.x : i < 4 ? q.y : i < 6 ? q.z : q.w;
+    return Row<float>::Finite(
+        fma2(__half22float2(Pair(w)), make_float2(kLog2E, kLog2E), make_float2(-scaled, -scaled)));
   }
   static __device__ __forceinline__ float LogProb(float x, float m, float log_z) {
     return fmaf(Exponent(x, Scaled(m)), kLn2, -log_z);
@@ -642,17 +656,16 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       const float scaled = R::Scaled(st.m);
 #pragma unroll
       for (int u = 0; u < kVectors; ++u) {
-        float z = 0.0f, w = 0.0f;  // of one vector: longer sums lose less
+        float2 z = {0.0f, 0.0f}, w = {0.0f, 0.0f};  // of one vector: longer sums lose less
 #pragma unroll
-        for (int e = 0; e < kE; ++e) {
-          // Finite, so that a closed token's 0 * t is 0.
-          const float t = fmaxf(R::Exponent(R::At(q[u], e), scaled), -16384.0f);
-          const float p = Exp2Approx(t);
-          z += p;
-          w = fmaf(p, t, w);
+        for (int e = 0; e < kE; e += 2) {
+          const float2 t = R::Exponents(q[u], e, scaled);
+          const float2 p = make_float2(Exp2Approx(t.x), Exp2Approx(t.y));
+          z = add2(z, p);
+          w = fma2(p, t, w);
         }
-        st.z += z;
-        st.w += w;
+        st.z += z.x + z.y;
+        st.w += w.x + w.y;
       }
     }
     if (ranks) {
@@ -841,7 +854,8 @@ void LaunchLogprobs(const LogprobArgs& a, cudaStream_t stream) {
   // Few rows: up to eight CTAs of a cluster share one, while each has vectors
   // for all of its threads and they fit the SMs twice over, or, with four
   // chunks for each and more, four times (an SM holds four).  One row of
-  // 151,936 floats: 13.8 us with eight CTAs, 16 with sixteen; 100 such rows:
+  // 151,936 floats, with CTAs of 256 threads: 17.5 us with eight of them, 19.6
+  // with sixteen (eight of 512 threads: 12.6); 100 such rows:
   // 22.3 us with four, 26.1 us with two; 64 rows of 32,000: 10.5 us with four,
   // 13.7 us with eight.
   constexpr int kVector = Row<T>::kN;
