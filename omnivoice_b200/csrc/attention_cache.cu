@@ -889,7 +889,7 @@ __global__ void __launch_bounds__(kStreamThreads + 128, 1)
 // A softmax step takes 64 keys of a tile and S has two buffers for each
 // warpgroup, so that the S of the next 64 keys is there when it starts: with
 // one S of 128 keys the softmax and the products of a row tile took turns
-// (215 us for the case below, 197 with the two buffers).  The products are
+// (215 us for the case below, 205 with the two buffers).  The products are
 // issued by the elected thread of a converged warp: from a divergent branch
 // each instruction cost about 100 cycles, of 64 that the tensor core needs
 // (324 us with these 48 products a key tile, 240 with 32 of 128 keys).
