@@ -12,7 +12,7 @@
 //
 // Measured on one B200: the audio head's 500 rows of 8 x 1,025 float32 values
 // (16.6 MB) 8.0 us; 512 half rows of 151,936 values (156 MB) with 20
-// alternatives 52 us, 3.0 TB/s: not the reading but about 13 instructions for
+// alternatives 52 us, 3.0 TB/s: not the reading but about 14 instructions for
 // a value bound it (6 for the sums and the rank, the rest for alternatives and
 // what a chunk costs; with the sums' operations one by one instead of in pairs,
 // 56 us); one float32 row of that length 12.6 us, its clusters' barriers and
