@@ -299,7 +299,8 @@ int ov_kv_cache_read(const ov_kv_cache* cache, const int32_t* cu_rows, const int
  * with a smaller one or NULL each row runs on one CTA.  Zero it once before
  * its first use: every call leaves its counters zero, so calls of any shapes
  * may share a workspace that is large enough for each.  Calls sharing one
- * must not overlap, captured ones included. */
+ * must not overlap, captured ones included.  The size is 0 for a call that
+ * needs none, and for sizes that the call refuses. */
 int ov_attention_kv_cache(const ov_kv_cache* cache, const uint16_t* q, size_t ld_q, size_t rows,
                           const int32_t* cu_rows, size_t max_rows, const int32_t* lengths,
                           size_t max_length, size_t heads, int causal, float scale, uint16_t* out,

@@ -1668,6 +1668,18 @@ void EncodeCodesMap(CUtensorMap* map, const int8_t* codes, const ov_kv_cache* ca
                     kCacheHeadDim, static_cast<uint32_t>(box_rows), swizzle);
 }
 
+// What both entry points refuse, so that no plan overflows.
+void RequireSizes(const ov_kv_cache* cache, size_t rows, size_t max_rows, size_t max_length,
+                  size_t heads) {
+  OV_REQUIRE(heads > 0 && heads % cache->kv_heads == 0, "heads must be a multiple of kv_heads");
+  OV_REQUIRE(heads <= 1024, "more than 1024 heads");
+  OV_REQUIRE(rows < (size_t{1} << 31), "rows must stay below 2^31");
+  OV_REQUIRE(max_length <= cache->max_pages * cache->page_tokens,
+             "max_length exceeds the page table");
+  OV_REQUIRE(std::min(max_rows, rows) <= ((size_t{1} << 31) - 512) / heads,
+             "max_rows * heads must stay below 2^31");
+}
+
 }  // namespace
 }  // namespace ovb
 
@@ -1679,8 +1691,10 @@ size_t ov_attention_kv_cache_workspace_bytes(const ov_kv_cache* cache, size_t ro
                                              size_t max_rows, size_t max_length, size_t heads) {
   size_t bytes = 0;
   const int status = Guard("ov_attention_kv_cache_workspace_bytes: ", [&] {
-    OV_REQUIRE(cache != nullptr && cache->kv_heads > 0, "cache");
-    OV_REQUIRE(heads > 0 && heads % cache->kv_heads == 0, "heads must be a multiple of kv_heads");
+    OV_REQUIRE(cache != nullptr && cache->kv_heads > 0 && cache->kv_heads <= 1024 &&
+                   cache->num_seqs <= 65535,
+               "cache");
+    RequireSizes(cache, rows, max_rows, max_length, heads);
     if (std::min(max_rows, rows) == 0 || cache->num_seqs == 0) return;
     const StreamPlan plan = PlanStream(cache, std::min(max_rows, rows), max_length, heads);
     const size_t parts = plan.rows > 0
@@ -1698,16 +1712,10 @@ int ov_attention_kv_cache(const ov_kv_cache* cache, const uint16_t* q, size_t ld
                           ov_stream_t stream) {
   return Guard("ov_attention_kv_cache: ", [&] {
     const CacheView c = ViewCache(cache);
-    OV_REQUIRE(heads > 0 && heads % cache->kv_heads == 0, "heads must be a multiple of kv_heads");
-    OV_REQUIRE(heads <= 1024, "more than 1024 heads");
+    RequireSizes(cache, rows, max_rows, max_length, heads);
     OV_REQUIRE(std::isfinite(scale) && scale > 0.0f, "scale must be positive and finite");
-    OV_REQUIRE(rows < (size_t{1} << 31), "rows must stay below 2^31");
-    OV_REQUIRE(max_length <= cache->max_pages * cache->page_tokens,
-               "max_length exceeds the page table");
     OV_REQUIRE(ld_q % 8 == 0 && ld_q >= heads * kCacheHeadDim, "q stride");
     OV_REQUIRE(ld_out % 8 == 0 && ld_out >= heads * kCacheHeadDim, "out stride");
-    OV_REQUIRE(std::min(max_rows, rows) <= ((size_t{1} << 31) - 512) / heads,
-               "max_rows * heads must stay below 2^31");
     if (rows == 0 || max_rows == 0 || c.num_seqs == 0) return;
     RequireAligned(q, 16, "q");
     RequireAligned(out, 16, "out");

@@ -256,6 +256,17 @@ def test_host_memory_is_refused():
         gpu.write(host, host, [4], [0])
 
 
+@pytest.mark.parametrize("change", [
+    dict(rows=2 ** 63, max_rows=2 ** 63), dict(rows=2 ** 40, max_rows=2 ** 40), dict(heads=2 ** 20),
+    dict(num_seqs=2 ** 63), dict(max_length=2 ** 60), dict(kv_heads=0), dict(heads=3)])
+def test_no_workspace_size_for_calls_that_are_refused(change):
+    args = dict(rows=40, max_rows=40, max_length=64, heads=4, num_seqs=1, kv_heads=2) | change
+    d = N.KvCache(kv_heads=args["kv_heads"], num_seqs=args["num_seqs"], head_dim=D, page_tokens=16,
+                  pages=4, max_pages=4)
+    assert N.lib().ov_attention_kv_cache_workspace_bytes(
+        ctypes.byref(d), args["rows"], args["max_rows"], args["max_length"], args["heads"]) == 0
+
+
 # ---------------------------------------------------------------- attention
 
 def filled(seqs, page, kv, lengths, g, page_sizes=False, extra=2):
