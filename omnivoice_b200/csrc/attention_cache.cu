@@ -1486,8 +1486,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     // even and the odd key tiles' parts of one tile: each takes half of the
     // columns, the other's half comes through shared memory (every MMA is
     // done by then, so the rings are idle).  Columns here: [col0, col0 + 32 n).
+    // A warpgroup without units has no MMA to wait for, but its query tile still
+    // takes both warpgroups' copies: its zeros go there behind all of them.
     if (units > 0)
       ok = ok && mbar_wait(&s.s_full[g][(units - 1) & 1], static_cast<uint32_t>(((units - 1) >> 1) + 1) & 1u, a.err);
+    else
+      ok = ok && mbar_wait(&s.q_full, 0, a.err);
     if (!pair) named_barrier(1, 256);
     __syncwarp();
     tc_fence_after_sync();

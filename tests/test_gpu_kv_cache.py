@@ -457,6 +457,26 @@ def test_no_tokens_at_all(n):
     assert (out == 0).all()
 
 
+@pytest.mark.parametrize("n", [129, 200, 256, 300, 513])
+@pytest.mark.parametrize("causal", [False, True])
+def test_rows_that_see_nothing_in_pairs_of_row_tiles(n, causal):
+    """Both row tiles of a CTA, or the first of them, without a token: zeros,
+    whatever the queries hold, in every launch."""
+    g = torch.Generator().manual_seed(n + causal)
+    lengths = ([0, 1, n - 129, n - 128, n - 127, n] * 4)[:20]
+    kv, heads = 4, 4  # 80 items of at least two tiles: more than single tiles fill a GPU with
+    check_attention(filled(20, 64, kv, lengths, g), [n] * 20, lengths, heads, causal, g)
+    gpu = GpuCache(filled(20, 64, kv, [0] * 20, g))
+    rows = 20 * n
+    q = torch.full((rows, heads * D), 7.0, dtype=torch.float16, device="cuda")
+    ws = gpu.workspace(rows, n, 0, heads)
+    for _ in range(8):
+        out = torch.full_like(q, 5.0)
+        gpu.attend(q, [n] * 20, [0] * 20, heads, causal, 0.1, out, ws)
+        torch.cuda.synchronize()
+        assert (out == 0).all()
+
+
 @pytest.mark.parametrize("n,heads,length,page", [(1, 2, 1_300_001, 16), (40, 1, 200_003, 64)])
 def test_a_very_long_history(n, heads, length, page):
     """Against float64 on the GPU, in pieces."""
