@@ -58,10 +58,12 @@ struct CacheAttnArgs {
   uint32_t* err;
 };
 
-// Stands for a value scale below it, 0 above all: such codes add nothing
-// that a half could hold (127 * 2^-31 is its least value), but their tokens
-// count in the denominator.  Below the least scale of a nonzero half page.
-constexpr float kLeastScale = 0x1.0p-31f;
+// Stands for a value scale below it, 0 above all, whose log2 the exponent
+// could not take: such codes add nothing that a half could hold (128 * 2^-33
+// is a quarter of the least one and rounds to 0, as what they stand for does),
+// but their tokens count in the denominator.  The least scale that a page of
+// halves is written with is 2^-24 / 127, four times as large.
+constexpr float kLeastScale = 0x1.0p-33f;
 
 // log2 and inverse of a value scale.  A NaN one (or a negative one, which
 // none is) makes the exponent NaN where it is seen, and must not reach a sum

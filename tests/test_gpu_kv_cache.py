@@ -575,6 +575,34 @@ def test_the_least_scales(n):
     check_attention(ref, [n], [100], 2, True, g, scale=1e-30)
 
 
+@pytest.mark.parametrize("n", [1, 12, 40, 300])
+@pytest.mark.parametrize("scale", [0.0, 1e-38, 1e-12, 2.0 ** -33, 2.0 ** -32])
+def test_value_scales_below_every_half(n, scale):
+    """Codes that are not zero under value scales so small that code * scale
+    rounds to 0 (128 * 2^-32 is half of the least half): zeros, as reading the
+    cache gives; and nothing beside a page of ordinary values."""
+    g = torch.Generator().manual_seed(n)
+    seqs = 50 if n == 300 else 2  # pairs of row tiles
+    lengths = [320, 90] * (seqs // 2)
+    ref = filled(seqs, 32, 1, lengths, g)
+    ref.codes[1][..., 5] = -127 if scale == 2.0 ** -32 else -128
+    ref.codes[1][..., 9] = 127
+    for s in range(seqs):
+        ref.scales[1][ref.table[s, :(lengths[s] + 31) // 32]] = scale
+    gpu = GpuCache(ref)
+    assert (gpu.read(lengths, [0] * seqs)[1] == 0).all()
+    q = torch.randn(seqs * n, D, generator=g).half().cuda()
+    out = torch.full_like(q, 5.0)
+    ws = gpu.workspace(seqs * n, n, 320, 1)
+    gpu.attend(q, [n] * seqs, lengths, 1, False, 0.1, out, ws)
+    torch.cuda.synchronize()
+    assert (out == 0).all()
+    # The page in the middle has ordinary values: the others only take their
+    # share of the probability.
+    ref.scales[1][ref.table[0, 4], 0] = 0.01
+    check_attention(ref, [n] * seqs, lengths, 1, False, g)
+
+
 def test_one_workspace_for_calls_of_any_shape_and_two_graphs():
     """A workspace goes from single tokens of few sequences to many, to
     blocks of rows and back, eagerly and in two graphs that share it."""
