@@ -286,7 +286,8 @@ int ov_kv_cache_read(const ov_kv_cache* cache, const int32_t* cu_rows, const int
  * q is half [rows][ld_q], head h in columns [h * head_dim, ...), out likewise
  * with ld_out (strides multiples of 8, pointers 16-byte aligned); cu_rows,
  * lengths device int32; max_rows and max_length bound rows and lengths of
- * one sequence (a longer length is cut there and reported); scale > 0.
+ * one sequence (a longer length is cut there and reported; max_length is at
+ * most max_pages * page_tokens and 2^31 - 1024); scale > 0.
  *
  * K and V enter the products as their codes, exact in half; the scales are
  * applied to the float32 scores and, as log2(value scale), inside the

@@ -1682,6 +1682,8 @@ void RequireSizes(const ov_kv_cache* cache, size_t rows, size_t max_rows, size_t
   OV_REQUIRE(rows < (size_t{1} << 31), "rows must stay below 2^31");
   OV_REQUIRE(max_length <= cache->max_pages * cache->page_tokens,
              "max_length exceeds the page table");
+  // Room for lengths rounded up to a key tile, and a loader's lanes behind it.
+  OV_REQUIRE(max_length <= (size_t{1} << 31) - 1024, "max_length must be at most 2^31 - 1024");
   OV_REQUIRE(std::min(max_rows, rows) <= ((size_t{1} << 31) - 512) / heads,
              "max_rows * heads must stay below 2^31");
 }

@@ -113,3 +113,17 @@ def test_nothing_to_do_is_no_error(native):
     assert read(native, cache(), max_rows=0) == 0
     assert attend(native, cache(), rows=0, q=None) == 0
     assert logprobs(native, rows=0, logits=None) == 0
+
+
+@pytest.mark.parametrize("page_tokens", [16, 32, 64, 128])
+@pytest.mark.parametrize("rows", [1, 3])
+def test_lengths_that_the_kernels_sums_would_overflow(native, page_tokens, rows):
+    """A page table may name almost 2^31 tokens; lengths stay so far below
+    that rounding them up to a step of the kernels holds in 32 bits."""
+    tokens = (1 << 31) - page_tokens
+    c = cache(page_tokens=page_tokens, max_pages=tokens // page_tokens)
+    for length in (tokens, (1 << 31) - 1023):
+        if length <= tokens:
+            refused(attend(native, c, rows=rows, max_length=length), "max_length")
+    # The largest length passes this check and fails a later one.
+    refused(attend(native, c, rows=rows, max_length=(1 << 31) - 1024, q=None), "q must not")
