@@ -1699,9 +1699,7 @@ size_t ov_attention_kv_cache_workspace_bytes(const ov_kv_cache* cache, size_t ro
                                              size_t max_rows, size_t max_length, size_t heads) {
   size_t bytes = 0;
   const int status = Guard("ov_attention_kv_cache_workspace_bytes: ", [&] {
-    OV_REQUIRE(cache != nullptr && cache->kv_heads > 0 && cache->kv_heads <= 1024 &&
-                   cache->num_seqs <= 65535,
-               "cache");
+    RequireShape(cache);
     RequireSizes(cache, rows, max_rows, max_length, heads);
     if (std::min(max_rows, rows) == 0 || cache->num_seqs == 0) return;
     const StreamPlan plan = PlanStream(cache, std::min(max_rows, rows), max_length, heads);

@@ -267,7 +267,7 @@ void RequireOnDevice(const ov_kv_cache* cache) {
   RequireOnDevice(cache->page_table, "page_table");
 }
 
-CacheView ViewCache(const ov_kv_cache* cache) {
+void RequireShape(const ov_kv_cache* cache) {
   OV_REQUIRE(cache != nullptr, "cache must not be null");
   OV_REQUIRE(cache->head_dim == kCacheHeadDim, "head_dim must be 128");
   const size_t p = cache->page_tokens;
@@ -279,6 +279,11 @@ CacheView ViewCache(const ov_kv_cache* cache) {
              "pages * kv_heads * page_tokens must stay below 2^31");
   OV_REQUIRE(cache->max_pages <= (size_t{1} << 31) / p - 1,
              "max_pages * page_tokens must stay below 2^31");
+}
+
+CacheView ViewCache(const ov_kv_cache* cache) {
+  RequireShape(cache);
+  const size_t p = cache->page_tokens;
   RequireAligned(cache->keys, 16, "keys");
   RequireAligned(cache->values, 16, "values");
   RequireAligned(cache->key_scales, 4, "key_scales");

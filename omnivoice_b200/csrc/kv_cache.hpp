@@ -28,6 +28,9 @@ struct CacheView {
   int32_t max_pages;
 };
 
+// Refuses sizes of a cache that the kernels do not take.
+void RequireShape(const ov_kv_cache* cache);
+
 // Checks a cache description (without its pointers' device) and returns the
 // kernels' view of it.
 CacheView ViewCache(const ov_kv_cache* cache);

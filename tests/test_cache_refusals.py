@@ -127,3 +127,17 @@ def test_lengths_that_the_kernels_sums_would_overflow(native, page_tokens, rows)
             refused(attend(native, c, rows=rows, max_length=length), "max_length")
     # The largest length passes this check and fails a later one.
     refused(attend(native, c, rows=rows, max_length=(1 << 31) - 1024, q=None), "q must not")
+
+
+@pytest.mark.parametrize("change,word", [(c, w) for c, w in CACHE if not any(
+    n in c for n in ("keys", "values", "key_scales", "value_scales", "page_table"))])
+def test_no_workspace_size_for_a_cache_that_is_refused(native, change, word):
+    """By the same check as the call's, whatever its pointers are."""
+    c = cache(**(dict(keys=None, page_table=None) | change))
+    assert native.ov_attention_kv_cache_workspace_bytes(ctypes.byref(c), 3, 3, 200, 4) == 0
+    assert word in N.last_error(), N.last_error()
+
+
+def test_no_workspace_size_without_a_cache(native):
+    assert native.ov_attention_kv_cache_workspace_bytes(None, 3, 3, 200, 4) == 0
+    assert "cache must not be null" in N.last_error()
