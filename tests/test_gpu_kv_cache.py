@@ -248,6 +248,46 @@ def test_what_only_the_device_sees_is_skipped_and_reported():
     assert not torch.equal(before[0], gpu.codes[0])
 
 
+def test_what_is_skipped_leaves_keys_values_and_scales():
+    """As above, for all that a write touches: codes and scales of keys and of
+    values, beside sequences that are written."""
+    g = torch.Generator().manual_seed(16)
+    table = torch.tensor([[0, 9, 1], [2, 3, -4], [4, 5, 10], [7, 8, 6]])
+    ref = Cache(10, 16, 2, table.clamp(0, 9))
+    ref.scales = [torch.rand(10, 2, generator=g) for _ in range(2)]
+    ref.table = table
+    gpu = GpuCache(ref)
+    gpu.desc.pages = 9  # page 9 lies behind the cache
+    x = torch.randn(120, 4 * D, generator=g).half()
+    d = x.cuda()
+    k, v = d[:, :2 * D], d[:, 2 * D:]
+
+    def wrote(seq, start, first, end):
+        for which in range(2):
+            ref.write(which, seq, start, x[first:end, which * 2 * D:(which + 1) * 2 * D].view(end - first, 2, D))
+
+    gpu.write(k, v, [40, 40, 3, 20], [0, 0, -1, 40])
+    assert device_errors() == N.OV_DEVICE_BAD_ARGUMENT
+    for call in ((0, 0, 0, 16), (0, 32, 32, 40), (1, 0, 40, 72), (3, 40, 83, 91)):
+        wrote(*call)
+    same_cache(ref, gpu)
+    # Bounds that decrease: the other sequences are written.
+    gpu.write(k, v, [5, -2, 9, 1], [0, 0, 0, 0], max_rows=9)
+    assert device_errors() == N.OV_DEVICE_BAD_ARGUMENT
+    for call in ((0, 0, 0, 5), (2, 0, 3, 12), (3, 0, 12, 13)):
+        wrote(*call)
+    same_cache(ref, gpu)
+    # More rows than there are, or than were announced, and a negative first row.
+    for counts, max_rows in (([200, 0, 0, 0], 200), ([12, 0, 0, 0], 11), ([-3, 3, 0, 0], 9)):
+        gpu.write(k, v, counts, [0, 0, 0, 0], max_rows=max_rows)
+        assert device_errors() == N.OV_DEVICE_BAD_ARGUMENT
+        same_cache(ref, gpu)
+    # What is read back of skipped tokens stays, keys and values.
+    for got in gpu.read([48], [0], fill=-3.0):
+        assert (got[16:32] == -3).all() and not (got[:16] == -3).any()
+    assert device_errors() == N.OV_DEVICE_BAD_ARGUMENT
+
+
 def test_host_memory_is_refused():
     g = torch.Generator().manual_seed(7)
     gpu = GpuCache(Cache(4, 16, 1, shuffled_table(1, 4, 0, g)))
@@ -551,6 +591,66 @@ def test_a_nan_page_that_only_later_rows_see(n, which):
     ref.scales[which][int(ref.table[0, 1]), 0] = 0.01  # not seen by these
     want, bound = reference(ref, q, [n], [length], 2, True, 0.1)
     assert ((got[:clean].double() - want[:clean]).abs() <= bound[:clean]).all()
+
+
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("page", [16, 64, 128])
+def test_a_nan_page_in_pairs_of_row_tiles(page, which):
+    """Each sequence has its NaN page elsewhere: before every row, inside what
+    only the later rows of the first tile see, or only the second tile."""
+    g = torch.Generator().manual_seed(page + which)
+    seqs, n, length = 50, 300, 400
+    ref = filled(seqs, page, 1, [length] * seqs, g)
+    used = -(-length // page)
+    at = [(s, s % used) for s in range(seqs)]
+    for s, j in at:
+        ref.scales[which][ref.table[s, j], 0] = float("nan")
+    q = torch.randn(seqs * n, D, generator=g).half()
+    gpu = GpuCache(ref)
+    out = torch.zeros(seqs * n, D, dtype=torch.float16, device="cuda")
+    gpu.attend(q.cuda(), [n] * seqs, [length] * seqs, 1, True, 0.1, out,
+               gpu.workspace(seqs * n, n, length, 1))
+    got = out.cpu().view(seqs, n, D)
+    for s, j in at:
+        ref.scales[which][ref.table[s, j], 0] = 0.01  # not seen by the rows that are compared
+    want, bound = reference(ref, q, [n] * seqs, [length] * seqs, 1, True, 0.1)
+    want, bound = want.view(seqs, n, D), bound.view(seqs, n, D)
+    for s, j in at:
+        clean = min(n, max(0, page * j - (length - n)))  # rows that end before the page
+        assert got[s, clean:].isnan().all()
+        assert ((got[s, :clean].double() - want[s, :clean]).abs() <= bound[s, :clean]).all()
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("page", [16, 64, 128])
+def test_bad_pages_in_pairs_of_row_tiles(page, causal):
+    """A page outside the cache, elsewhere in each sequence, counts as tokens
+    that nothing sees, for both row tiles."""
+    g = torch.Generator().manual_seed(page + causal)
+    seqs, n, length = 50, 300, 400
+    ref = filled(seqs, page, 1, [length] * seqs, g)
+    table, used = ref.table.clone(), -(-length // page)
+    for s in range(seqs):
+        ref.table[s, s % used] = (-1, ref.codes[0].shape[0], 2 ** 31 - 1)[s % 3]
+    q = torch.randn(seqs * n, D, generator=g).half()
+    gpu = GpuCache(ref)
+    out = torch.zeros(seqs * n, D, dtype=torch.float16, device="cuda")
+    gpu.attend(q.cuda(), [n] * seqs, [length] * seqs, 1, causal, 0.1, out,
+               gpu.workspace(seqs * n, n, length, 1))
+    torch.cuda.synchronize()
+    assert device_errors() == N.OV_DEVICE_BAD_ARGUMENT
+    got = out.cpu().double().view(seqs, n, D)
+    ref.table = table
+    token = torch.arange(length)
+    for s in range(seqs):
+        keep = token[token // page != s % used]
+        k, v = (ref.tokens(w, s, 0, length)[0][keep] for w in range(2))
+        pages = table[s][keep // page]
+        ends = length - n + 1 + torch.arange(n) if causal else torch.full((n,), length)
+        seen = (keep < ends[:, None]).sum(-1)
+        want, bound = attention(q[s * n:(s + 1) * n].double(), k, v, ref.scales[0][pages, 0].double(),
+                                ref.scales[1][pages, 0].double(), seen, 0.1)
+        assert ((got[s] - want).abs() <= bound).all()
 
 
 @pytest.mark.parametrize("n", [1, 50])
