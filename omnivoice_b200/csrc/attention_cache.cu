@@ -1310,8 +1310,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                       (token & ((1 << cache.page_shift) - 1));
       bool ok = true;
       for (int w = 0; w < 2 && ok; ++w) {
-        if (t > 0) ok = mbar_wait(&s.codes_empty[w], static_cast<uint32_t>(t - 1) & 1u, a.err);
-        if (lane < kSlabs) {
+        // The whole warp together: a lane that came late could find the barrier
+        // two phases on, by the others' arrivals.
+        if (t > 0) ok = WarpWait(&s.codes_empty[w], static_cast<uint32_t>(t - 1) & 1u, a.err);
+        if (lane < kSlabs && ok) {
           if (page >= 0 && lane * 16 % box == 0) {
             mbar_arrive_expect_tx(&s.codes_full[w], box * kCacheHeadDim);
             tma_load_2d(code_s + w * kCodeTile + lane * 16 * kCacheHeadDim, w == 0 ? &map_k : &map_v,
