@@ -461,8 +461,11 @@ __global__ void __launch_bounds__(kStreamThreads + 128, 1)
     uint64_t idle_since = 0;
     while (__any_sync(0xFFFFFFFFu, at < p1)) {
       const int stage = sent % kStages;
-      const bool ready = at < p1 && (sent < kStages ||
-                                     mbar_test_wait(&empty[stage], static_cast<uint32_t>(sent / kStages - 1) & 1u));
+      // Free, and what was copied there before has landed: a warp that gave up
+      // waiting for it frees the slot without.
+      const uint32_t used = static_cast<uint32_t>(sent / kStages - 1) & 1u;
+      const bool ready = at < p1 && (sent < kStages || (mbar_test_wait(&empty[stage], used) &&
+                                                        mbar_test_wait(&info[stage].full, used)));
       if (ready) {
         int now[2];
 #pragma unroll
@@ -510,6 +513,9 @@ __global__ void __launch_bounds__(kStreamThreads + 128, 1)
       }
     }
     cp_async_wait_all();
+    // No copy outlives the CTA.
+    for (int u = max(0, sent - kStages); u < sent; ++u)
+      (void)mbar_wait(&info[u % kStages].full, static_cast<uint32_t>(u / kStages) & 1u, a.err);
     return;
   }
   registers_grow<224>();
@@ -1310,9 +1316,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                       (token & ((1 << cache.page_shift) - 1));
       bool ok = true;
       for (int w = 0; w < 2 && ok; ++w) {
-        // The whole warp together: a lane that came late could find the barrier
-        // two phases on, by the others' arrivals.
-        if (t > 0) ok = WarpWait(&s.codes_empty[w], static_cast<uint32_t>(t - 1) & 1u, a.err);
+        // The whole warp together: a lane that came late could find a barrier
+        // two phases on, by the others' arrivals.  Landed, too: converters that
+        // gave up waiting for codes free them all the same.
+        const uint32_t used = static_cast<uint32_t>(t - 1) & 1u;
+        if (t > 0)
+          ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s.codes_empty[w], used, a.err) &&
+                                           mbar_wait(&s.codes_full[w], used, a.err));
         if (lane < kSlabs && ok) {
           if (page >= 0 && lane * 16 % box == 0) {
             mbar_arrive_expect_tx(&s.codes_full[w], box * kCacheHeadDim);
@@ -1337,6 +1347,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       __syncwarp();
       if (!__all_sync(0xFFFFFFFFu, ok)) break;
     }
+    // No copy outlives the CTA (behind a wait that ran out, all had its time).
+    if (nt > 0)
+      for (int w = 0; w < 2; ++w)
+        (void)mbar_wait(&s.codes_full[w], static_cast<uint32_t>(nt - 1) & 1u, a.err);
   } else if (warp >= kConvertWarp && warp < kLoadWarp) {
     const int ctid = tid - kConvertWarp * 32;
     bool ok = true;  // once a wait ran out, no other is begun
