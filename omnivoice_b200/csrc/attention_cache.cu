@@ -51,7 +51,6 @@ struct CacheAttnArgs {
   int rows;
   int max_rows;
   int max_length;
-  int heads;
   FastDiv group;  // heads / kv_heads
   int causal;
   float scale_log2;  // softmax scale * log2(e)
@@ -121,10 +120,12 @@ constexpr int kUnitTile = kUnit * kCacheHeadDim;  // bytes of K or V of a unit
 constexpr int kStreamWarps = 8;
 constexpr int kStreamThreads = kStreamWarps * 32;  // of the warps that compute
 // Units of a warp where items get CTAs of their own: more make a short item's
-// warps work longer, fewer split it over CTAs and add their join.  One token
-// of 8 kv heads over 300 / 1,500 / 8,192 tokens took 8.7 / 11.0 / 12.5 us with
-// 2, 8.6 / 12.2 / 13.3 with 3, 9.5 / 13.4 / 13.9 with 4; 16 sequences of up to
-// 700 tokens 12.6 us with 2, 10.5 with 3, 11.7 with 4.
+// warps work longer, fewer split it over CTAs and add their join.  3 is for
+// batches of short histories: 16 sequences of up to 700 tokens took 12.6 us
+// with 2, 10.5 with 3, 11.7 with 4, and a CTA's 768 tokens hold a prompt of
+// 705.  One sequence, whose items leave most of the GPU idle, is as fast or
+// faster with 2: 8 kv heads over 300 / 1,500 / 8,192 tokens 8.7 / 11.0 / 12.5
+// us with 2, 8.6 / 12.2 / 13.3 with 3, 9.5 / 13.4 / 13.9 with 4.
 constexpr int kMinUnits = 3;
 
 // Ring slot beside the codes: scales and pages of the unit's two 16-key
@@ -1761,7 +1762,6 @@ int ov_attention_kv_cache(const ov_kv_cache* cache, const uint16_t* q, size_t ld
     a.rows = static_cast<int>(rows);
     a.max_rows = static_cast<int>(std::min(max_rows, rows));
     a.max_length = static_cast<int>(max_length);
-    a.heads = static_cast<int>(heads);
     a.causal = causal != 0;
     a.scale_log2 = scale * 1.4426950408889634f;
     a.err = DeviceErrorWord();

@@ -298,8 +298,9 @@ constexpr int kWarpKeys = 64;
 
 // The whole group sits in registers, value j in lane j % 32: a load, a
 // maximum, an exponential, two comparisons and a handful of sums for a value.
-// What bounds it is the instructions (about 20 for a value, with what a row
-// costs once), with the loads' latency hidden by the SM's 32 warps.
+// What bounds it is the instructions (35 for a value of 8 x 1,025 with five
+// alternatives, what a row costs once among them; 12 bytes of a thread spill),
+// with the loads' latency hidden by the SM's 32 warps.
 template <typename T, int kPer>
 __global__ void __launch_bounds__(kWarps * 32, kPer <= 33 ? 4 : 2)
     logprobs_warp_kernel(const LogprobArgs a) {
