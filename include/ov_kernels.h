@@ -263,7 +263,8 @@ typedef struct {
  * current end) is allowed.  Slots behind the last written token keep their
  * codes.  A page with a NaN or an infinity among its rows gets a NaN scale,
  * hence reads back as NaN, until it is rewritten from its first slot.
- * A page may be written by one sequence of a call only. */
+ * A page may be written once in a call: by one sequence, at one place of its
+ * table. */
 int ov_kv_cache_write(const ov_kv_cache* cache, const uint16_t* k, size_t ld_k, const uint16_t* v,
                       size_t ld_v, size_t rows, const int32_t* cu_rows, const int32_t* starts,
                       size_t max_rows, ov_stream_t stream);

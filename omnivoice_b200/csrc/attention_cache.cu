@@ -112,8 +112,10 @@ __device__ __forceinline__ int CheckLength(const CacheAttnArgs& a, int length) {
 // (303 MB of codes): 58 us, 5.2 TB/s; in its middle the kernel reads at the
 // rate of a plain copy, the rest is about 4 us before the first keys arrive
 // (lengths, page table, TMA, each waiting for the one before) and 4 us of
-// joins.  4 sequences of 65,537 tokens, 16 heads over 2 (134 MB): 36 us.  One
-// token over 705: 10 us, all of it such waits.
+// joins.  4 sequences of 65,537 tokens, 16 heads over 2 (134 MB): 36 us, of
+// which 18 for 15 units a warp, 5 before the first keys and 7 of joins.  One
+// token over 705: 10 us, all of it such waits.  Spills 36 bytes a thread (52
+// with two blocks of 8 rows).
 
 constexpr int kUnit = 32;               // keys
 constexpr int kUnitTile = kUnit * kCacheHeadDim;  // bytes of K or V of a unit
@@ -908,8 +910,8 @@ __global__ void __launch_bounds__(kStreamThreads + 128, 1)
 // probabilities' way back 1,300; the MMAs take 1,280 beside that, K's and V's
 // conversion 1,600 a tile), and by what comes before and after a CTA's key
 // tiles, 7,400 and 3,100 cycles.  Measured on one B200: 16 causal sequences of
-// up to 2,175 rows, 16 heads over 8: 197 us, 632 TFLOP/s of what is seen; 375
-// rows over 705 tokens: 15.5 us, where a CTA sees 2 key tiles.
+// up to 2,175 rows, 16 heads over 8: 198 us, 630 TFLOP/s of what is seen; 375
+// rows over 705 tokens: 15.7 us, where a CTA sees 2 key tiles.
 //
 // Registers: 512 threads start with 128 each; the softmax warpgroups take 152,
 // the other two keep 104.
